@@ -232,6 +232,162 @@ PTOWSP_API int ptowsp_cuda_paged_decode_noalloc(const void* q, const void* k_cac
 PTOWSP_API size_t ptowsp_cuda_noalloc_scratch_bytes(int num_requests, int num_kv_heads, int group, int max_pages,
                                                     int page_size);
 
+/* ------------------------------------------------------------------------- */
+/* Serving operators around a paged KV cache held in 8 bits.  No counterpart   */
+/* in the reference.  A serving step is                                        */
+/*   reserve (pages and slots of the new tokens) -> append (write their K, V)  */
+/*   -> attention (read the cache) -> sample (logits to tokens),               */
+/* all on the caller's stream with no host read in between.                    */
+/*                                                                             */
+/* Every pointer is device memory of the calling thread's current device       */
+/* except the argument structs.  The calls check sizes and pointers, launch on */
+/* `stream` (NULL: the default stream), return at once, allocate nothing and   */
+/* keep nothing, so they can be captured into a graph (after one call outside, */
+/* which loads their code).  What only the device can see goes to `status`, a  */
+/* device word that the caller zeroes (or NULL): the bits below are or'ed in,  */
+/* and the item in question is skipped, never accessed out of range.           */
+/* ------------------------------------------------------------------------- */
+
+enum ptowsp_dtype { PTOWSP_F32 = 0, PTOWSP_F16 = 1, PTOWSP_BF16 = 2 };
+enum ptowsp_kv8_format { PTOWSP_KV8_E4M3 = 0, PTOWSP_KV8_INT8 = 1 };
+
+enum ptowsp_serving_status {
+    PTOWSP_SERVING_PAGE = 1,    /* a page id or slot outside the cache */
+    PTOWSP_SERVING_LENGTH = 2,  /* a length that is negative, or beyond the page table */
+    PTOWSP_SERVING_REFUSED = 4, /* a request's new tokens found no room (pages, table or token list) */
+    PTOWSP_SERVING_RING = 8,    /* the free-page ring's state is inconsistent (too many pages given back) */
+    PTOWSP_SERVING_TIMEOUT = 16 /* a bounded wait inside a kernel gave up: the output is not complete */
+};
+
+/* Gives pages to the new tokens of `requests` requests and takes back the pages of those that ended.
+ *   page_table  i32 [requests][max_pages], rows `table_stride` apart; the new pages' entries are written
+ *   kv_len      i32 [requests]  tokens each request has in the cache
+ *   new_tokens  i32 [requests]  tokens to come; negative: the request ended
+ *   free_ring   i32 [ring_size] free page ids at places head .. tail - 1, modulo ring_size
+ *   free_state  i64 [2]         (head, tail), 0 <= tail - head <= ring_size
+ * Requests are served in order; one whose pages the ring does not have, or whose tokens pass the table or
+ * `max_tokens`, is refused (its length stays, its slots are -1).  Pages of ended requests go behind the tail and are
+ * given out from the next call on.  Results, none aliasing an input:
+ *   slots       i64 [max_tokens]   page * page_size + offset of each new token, request after request; -1: none
+ *   positions   i32 [max_tokens]   its position in its request; -1: none
+ *   q_start     i32 [requests + 1] prefix sums of the new tokens (refused requests keep their place)
+ *   kv_len_out  i32 [requests], free_state_out i64 [2], granted u8 [requests]
+ * page_size: a power of two, 1 .. 65536; requests at most 16384.  The call can be repeated on the same inputs. */
+typedef struct ptowsp_reserve_args {
+    int32_t* page_table;
+    int64_t table_stride;
+    int32_t max_pages, page_size, requests, reserved0;
+    const int32_t* kv_len;
+    const int32_t* new_tokens;
+    int32_t* free_ring;
+    int64_t ring_size;
+    const int64_t* free_state;
+    int64_t* slots;
+    int32_t* positions;
+    int64_t max_tokens;
+    int32_t* q_start;
+    int32_t* kv_len_out;
+    int64_t* free_state_out;
+    uint8_t* granted;
+    int32_t* status;
+} ptowsp_reserve_args;
+PTOWSP_API int ptowsp_cuda_reserve_pages(const ptowsp_reserve_args* args, void* stream);
+
+/* A paged KV cache in 8 bits: codes [num_pages][page_size][num_kv_heads][head_dim] of K and of V with any page, token
+ * and head strides (in elements; multiples of 16, codes 16-byte aligned, head_dim contiguous), and one f32 scale per
+ * page and head, [num_pages][num_kv_heads]: value = code * scale.  Scales are within 2^-60 .. 2^60.
+ * page_size: 16, 32, 64 or 128; head_dim: 64 or 128. */
+typedef struct ptowsp_kv8_cache {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t k_page_stride, k_token_stride, k_head_stride;
+    int64_t v_page_stride, v_token_stride, v_head_stride;
+    int64_t num_pages;
+    int32_t page_size, num_kv_heads, head_dim;
+    int32_t format; /* ptowsp_kv8_format */
+} ptowsp_kv8_cache;
+
+/* Writes new K and V rows into the cache.  k, v: [tokens][num_kv_heads][head_dim] of `dtype`, strides in elements,
+ * rows 16-byte aligned.  slots: i64 [tokens], page * page_size + offset, -1: skip; the slots of one page stand next to
+ * each other in ascending order (as ptowsp_cuda_reserve_pages makes them), and no page belongs to two requests.
+ * For each touched page and head, from the largest finite |x| of its new tokens:
+ *   need  = the smallest power of two s with max <= 448 s (e4m3), or max * (1 / 127) in f32 (int8), within 2^-60 .. 2^60
+ *   scale = max(need, old), or need alone if the page's token 0 is among the new ones (the page is new)
+ * and where it grew, the page's other codes are rounded again to the new scale.  code = round to nearest even of
+ * x / scale, clamped to the largest code; NaN is written as 0. */
+typedef struct ptowsp_kv8_append_args {
+    const void* k;
+    const void* v;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    const int64_t* slots;
+    int64_t tokens;
+    int32_t dtype; /* ptowsp_dtype */
+    int32_t reserved0;
+    int32_t* status;
+} ptowsp_kv8_append_args;
+PTOWSP_API int ptowsp_cuda_kv8_append(const ptowsp_kv8_cache* cache, const ptowsp_kv8_append_args* args, void* stream);
+
+/* Causal attention of the newest tokens of each request over its cached tokens.
+ *   q, out      [tokens][num_heads][head_dim] of `dtype` (f16 or bf16), strides in elements, rows 16-byte aligned;
+ *               head i reads KV head i / (num_heads / num_kv_heads)
+ *   lse         f32 [tokens][num_heads], or NULL: log of the sum of the exponentials
+ *   page_table  i32 [requests][max_pages], rows `table_stride` apart
+ *   kv_len      i32 [requests], the new tokens included
+ *   q_start     i32 [requests + 1], q rows of request r: q_start[r] .. q_start[r + 1] - 1; NULL: row r
+ *   max_q       the most rows that any request has
+ *   window      > 0: a row sees its own token and the window - 1 before it; 0: all before it
+ * Row j of nq sees the keys t <= kv_len - nq + j.  A row that sees none gets zeros and lse = -inf.  A page id
+ * outside the cache hides its tokens.  `workspace`: ptowsp_cuda_kv8_attention_workspace bytes, 256-byte aligned,
+ * contents irrelevant, used until the call's work on the stream is done. */
+typedef struct ptowsp_kv8_attention_args {
+    const void* q;
+    void* out;
+    float* lse;
+    int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+    const int32_t* page_table;
+    int64_t table_stride;
+    const int32_t* kv_len;
+    const int32_t* q_start;
+    int64_t tokens;
+    int32_t max_pages, requests, num_heads, max_q, window;
+    int32_t dtype; /* ptowsp_dtype */
+    float scale;   /* of the scores, before the softmax */
+    int32_t reserved0;
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t* status;
+} ptowsp_kv8_attention_args;
+PTOWSP_API int ptowsp_cuda_kv8_attention(const ptowsp_kv8_cache* cache, const ptowsp_kv8_attention_args* args,
+                                         void* stream);
+PTOWSP_API size_t ptowsp_cuda_kv8_attention_workspace(const ptowsp_kv8_cache* cache,
+                                                      const ptowsp_kv8_attention_args* args);
+
+/* One token per row of logits [rows][vocab] (f32, f16 or bf16; rows `row_stride` elements apart), from one uniform
+ * random number u[row] in [0, 1) each.  With the row's largest logit M, w_i = exp((x_i - M) / temperature), taken as a
+ * whole number of 2^-40 (so its sums do not depend on their order).  Ordered by falling logit, ties by rising index,
+ * the candidates are cut to the first top_k, to w_i >= min_p, and then to the shortest prefix that holds top_p of what
+ * is left; the token is the first candidate, by index, at which the running sum of w passes u times the sum.
+ * NULL settings, top_k <= 0, top_p >= 1 and min_p <= 0 cut nothing; temperature 0 (or below) takes the largest logit,
+ * of several the first.  NaN counts as -inf; -inf is never taken; a row of nothing else gives token -1.
+ *   token i32 [rows], logprob f32 [rows] or NULL: log of the token's share of the candidates' sum. */
+typedef struct ptowsp_sample_args {
+    const void* logits;
+    int64_t row_stride;
+    int32_t rows, vocab;
+    int32_t dtype; /* ptowsp_dtype */
+    int32_t reserved0;
+    const float* u;
+    const float* temperature; /* per row; NULL: 1 */
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    int32_t* token;
+    float* logprob;
+} ptowsp_sample_args;
+PTOWSP_API int ptowsp_cuda_sample_tokens(const ptowsp_sample_args* args, void* stream);
+
 /* Number of CUDA devices visible to this library (0 without a GPU). */
 PTOWSP_API int ptowsp_cuda_device_count(void);
 

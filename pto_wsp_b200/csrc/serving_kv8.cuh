@@ -1,0 +1,50 @@
+// Conversions of the 8-bit cache codes, shared by its writer and its readers.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/ptowsp_cuda.h"
+
+namespace ptowsp::dev {
+
+// Two e4m3 codes (low half of w) as two f16: exact, f16 has every e4m3 value.
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(w));
+    return r;
+}
+
+// Bytes 0, 1 -> lo and bytes 2, 3 -> hi as f16 pairs, exactly.  int8: the byte with its sign flipped is the low
+// mantissa byte of 1024 + (code + 128), from which 1152 is taken.
+template <int FMT>
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if (FMT == PTOWSP_KV8_E4M3) {
+        lo = e4m3x2_f16x2(w);
+        hi = e4m3x2_f16x2(w >> 16);
+    } else {
+        w ^= 0x80808080u;
+        lo = __byte_perm(w, 0x64646464u, 0x4140);
+        hi = __byte_perm(w, 0x64646464u, 0x4342);
+        const __half2 bias = __floats2half2_rn(1152.f, 1152.f);
+        *reinterpret_cast<__half2*>(&lo) = __hsub2(*reinterpret_cast<__half2*>(&lo), bias);
+        *reinterpret_cast<__half2*>(&hi) = __hsub2(*reinterpret_cast<__half2*>(&hi), bias);
+    }
+}
+
+template <int FMT>
+__device__ __forceinline__ void decode4(uint32_t w, float (&f)[4]) {
+    uint32_t lo, hi;
+    codes_f16<FMT>(w, lo, hi);
+    const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo));
+    const float2 b = __half22float2(*reinterpret_cast<__half2*>(&hi));
+    f[0] = a.x;
+    f[1] = a.y;
+    f[2] = b.x;
+    f[3] = b.y;
+}
+
+}  // namespace ptowsp::dev
