@@ -4,6 +4,7 @@
 
 #include <cuda_runtime_api.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/ptowsp_cuda.h"
@@ -13,6 +14,23 @@ namespace ptowsp::dev {
 constexpr int kReserveMaxRequests = 16384;  // two words of shared memory each
 constexpr float kKv8MinScale = 8.673617379884035e-19f;  // 2^-60
 constexpr float kKv8MaxScale = 1152921504606846976.f;   // 2^60
+
+// A kernel's opt-in to more than 48 KB of dynamic shared memory, asked for once per device.
+class SmemOptIn {
+    std::atomic<uint64_t> done_{0};
+
+public:
+    cudaError_t once(const void* kernel, int bytes) {
+        int device = 0;
+        cudaError_t e = cudaGetDevice(&device);
+        if (e != cudaSuccess) return e;
+        const uint64_t bit = uint64_t{1} << (device & 63);
+        if (device < 64 && (done_.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess && device < 64) done_.fetch_or(bit, std::memory_order_relaxed);
+        return e;
+    }
+};
 
 struct ReserveArgs {
     int32_t* page_table;

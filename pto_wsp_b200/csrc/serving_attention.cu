@@ -17,6 +17,7 @@
 
 #include "serving.hpp"
 #include "serving_kv8.cuh"
+#include "tc_common.cuh"
 
 namespace ptowsp::dev {
 
@@ -25,23 +26,21 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kTile = 32;                 // tokens per warp and step
 constexpr int kUnit = kWarps * kTile;     // tokens per CTA and step: the grain in which work is dealt out
-constexpr int kStages = 3;
+constexpr int kSlots = 3;                  // tiles of K or V that a warp's ring holds
 constexpr int kThreads = kWarps * 32;
-constexpr int kCtasPerSm = 2;
+constexpr float kNone = -1.7e38f;         // M before the first visible key: below every exponent, yet finite
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// CTAs per SM: with one fragment of q rows 128 registers do, and 16 warps hide each other's latencies
+__host__ __device__ constexpr int ctas_per_sm(int nb) { return nb == 1 ? 4 : nb == 2 ? 3 : 2; }
+
+// A box of a page's codes (D bytes of one head, some tokens) into shared memory; its bytes count on `bar`.
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, int head, int token, int page,
+                                              uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(head), "r"(token), "r"(page), "r"(bar)
+        : "memory");
 }
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -72,6 +71,11 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+__device__ __forceinline__ float rcp_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 __device__ __forceinline__ float log2_approx(float x) {
     float r;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -86,7 +90,7 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 // Dealing out the work.  A request has `tiles` tiles of q rows for each KV head, and every one of these tasks takes
 // `units` steps of kUnit tokens.  The steps of all tasks stand in one line (request, tile, head, step), and CTA c of n
 // takes the c-th n-th of it, so all CTAs read the same amount whatever the lengths are.  A task that this cuts leaves
-// one partial result in each CTA it touches, which a second launch joins.
+// one partial result in each CTA it touches, and the last of these CTAs to finish joins them.
 // ---------------------------------------------------------------------------
 
 struct Request {
@@ -128,11 +132,25 @@ __device__ __forceinline__ Request request_at(const AttendArgs& a, int r, int* f
     return q;
 }
 
+// a / b for a >= 0, b > 0: 64-bit division is a long routine, and what is divided here nearly always fits 32 bits.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+
 // The steps of all requests, and for a place in their line the request that holds it and the steps before that.
 struct Deal {
-    int64_t total;   // steps in all
-    int64_t ctas;    // CTAs that share them
-    int per;         // requests per thread of the scan
+    int64_t total;        // steps in all
+    int64_t ctas;         // CTAs that share them
+    int64_t share, rest;  // steps of each, and the first CTAs that have one more
+    int per;              // requests per thread of the scan
+
+    __device__ __forceinline__ int64_t start(int64_t c) const { return c * share + (c < rest ? c : rest); }
+    // the CTA that has step i
+    __device__ __forceinline__ int64_t owner(int64_t i) const {
+        const int64_t big = rest * (share + 1);
+        return i < big ? quotient(i, share + 1) : rest + quotient(i - big, share);
+    }
 };
 
 template <int ROWS>
@@ -161,12 +179,9 @@ __device__ Deal deal_out(const AttendArgs& a, int ctas, int64_t* sums, int* flag
     __syncthreads();
     d.total = sums[kThreads - 1];
     d.ctas = d.total < ctas ? (d.total > 0 ? d.total : 1) : ctas;
+    d.share = quotient(d.total, d.ctas);
+    d.rest = d.total - d.share * d.ctas;
     return d;
-}
-
-// First step of CTA c.
-__device__ __forceinline__ int64_t deal_start(const Deal& d, int64_t c) {
-    return c * (d.total / d.ctas) + (c < d.total % d.ctas ? c : d.total % d.ctas);
 }
 
 struct Place {
@@ -192,55 +207,194 @@ __device__ Place find_place(const AttendArgs& a, const Deal& d, const int64_t* s
         if (at < before + n) break;
         before += n;
     }
-    p.task = (at - before) / p.q.units;
-    p.unit = (at - before) % p.q.units;
+    p.task = quotient(at - before, p.q.units);
+    p.unit = at - before - p.task * p.q.units;
     return p;
 }
 
+// The workspace: arrival counters, one per CTA, then two partial results per CTA.
+constexpr int kMaxSms = 512;
+constexpr size_t kArrivals = kMaxSms * 4 * sizeof(int);
+// A partial result: [rows][M, l], then [rows][D] of O.
 template <int D, int NB>
 constexpr size_t partial_floats() { return static_cast<size_t>(8 * NB) * (D + 2); }
 
-template <int D, int NB>
-constexpr int attend_smem() {
-    const int stage = kTile * D * 2 + 32;  // K and V codes, 4 scales
-    const int ring = kWarps * kStages * stage;
-    const int q = 8 * NB * (2 * D + 32);
-    return ring + q + 8 * NB * 8 + kWarps * 8 * NB * 8;
+// Divides V dims of a finished row by its sum and stores them, and the row's lse where `first`.
+template <int V>
+__device__ __forceinline__ void store_row(const AttendArgs& a, const Request& q, int head, int flat, int dim,
+                                          const float (&x)[V], float m, float sum, bool first) {
+    const int64_t tok = q.row0 + flat / a.group;
+    const int hq = head * a.group + flat % a.group;
+    const bool any = sum > 0.f || sum != sum;  // NaN goes through; a row that saw no key is zero
+    const float r = any ? 1.f / sum : 0.f;
+    const int64_t off = tok * a.out_token_stride + hq * a.out_head_stride + dim;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        if (a.dtype == PTOWSP_F16) static_cast<__half*>(a.out)[off + k] = __float2half_rn(x[k] * r);
+        else static_cast<__nv_bfloat16*>(a.out)[off + k] = __float2bfloat16_rn(x[k] * r);
+    }
+    if (first && a.lse) a.lse[tok * a.heads + hq] = any ? (m + log2f(sum)) * 0.6931471805599453f : -INFINITY;
 }
+
+// Joins the `pieces` partial results of a task: `first` is the one that CTA c0 left in its second place, the others
+// stand in the first places of CTA c0 + 1 and on.  Few pieces: a warp per row; many (a long history of one request):
+// the warps share the pieces of four rows at a time, so that enough loads are under way.  `x_smem`: [kWarps][4][D + 1].
+template <int D, int NB>
+__device__ void join_pieces(const AttendArgs& a, const Request& q, int head, int row_base, int rows, const float* first,
+                            int pieces, float* x_smem) {
+    constexpr int ROWS = 8 * NB, V = D / 32, R = 4;
+    constexpr int64_t kPiece = partial_floats<D, NB>();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const auto piece = [&](int i) { return first + (i == 0 ? 0 : (2 * i - 1) * kPiece); };
+    const auto top_of = [&](int row) {
+        float m = kNone;
+        for (int i = lane; i < pieces; i += 32) m = fmaxf(m, __ldcg(piece(i) + row * 2));
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+        return m;
+    };
+    if (pieces <= 2 * kWarps) {
+        for (int row = warp; row < rows; row += kWarps) {
+            const float m = top_of(row);
+            float x[V], sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < V; ++k) x[k] = 0.f;
+#pragma unroll 4
+            for (int i = 0; i < pieces; ++i) {
+                const float* o = piece(i);
+                const float f = exp2_approx(__ldcg(o + row * 2) - m);
+                sum = fmaf(f, __ldcg(o + row * 2 + 1), sum);
+#pragma unroll
+                for (int k = 0; k < V; ++k) x[k] = fmaf(f, __ldcg(o + 2 * ROWS + row * D + lane * V + k), x[k]);
+            }
+            store_row<V>(a, q, head, row_base + row, lane * V, x, m, sum, lane == 0);
+        }
+        return;
+    }
+    for (int row0 = 0; row0 < rows; row0 += R) {
+        float m[R], x[R][V], sum[R];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            m[j] = row0 + j < rows ? top_of(row0 + j) : kNone;
+            sum[j] = 0.f;
+#pragma unroll
+            for (int k = 0; k < V; ++k) x[j][k] = 0.f;
+        }
+#pragma unroll 2
+        for (int i = warp; i < pieces; i += kWarps) {
+            const float* st = piece(i) + row0 * 2;
+            const float* o = piece(i) + 2 * ROWS + row0 * D + lane * V;
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                if (row0 + j < rows) {
+                    const float f = exp2_approx(__ldcg(st + j * 2) - m[j]);
+                    sum[j] = fmaf(f, __ldcg(st + j * 2 + 1), sum[j]);
+#pragma unroll
+                    for (int k = 0; k < V; ++k) x[j][k] = fmaf(f, __ldcg(o + j * D + k), x[j][k]);
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            float* to = x_smem + (warp * R + j) * (D + 1);
+#pragma unroll
+            for (int k = 0; k < V; ++k) to[lane * V + k] = x[j][k];
+            if (lane == 0) to[D] = sum[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            if (j != warp || row0 + j >= rows) continue;
+            float y[V], l = 0.f;
+#pragma unroll
+            for (int k = 0; k < V; ++k) y[k] = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float* from = x_smem + (w * R + j) * (D + 1);
+                l += from[D];
+#pragma unroll
+                for (int k = 0; k < V; ++k) y[k] += from[lane * V + k];
+            }
+            store_row<V>(a, q, head, row_base + row0 + j, lane * V, y, m[j], l, lane == 0);
+        }
+    }
+}
+
+template <int D, int NB>
+struct Layout {
+    static constexpr int ROWS = 8 * NB;
+    static constexpr int kSlot = kTile * D;               // bytes of a tile of K or of V
+    static constexpr int QP = 2 * D + 32;                 // bytes between q rows: their 8-byte fragment loads hit all banks
+    static constexpr int kRing = kWarps * kSlots * kSlot;
+    static constexpr int kQ = kRing;                      // [ROWS] rows of QP bytes
+    static constexpr int kRow = kQ + ROWS * QP;           // [ROWS] factor, [ROWS] last visible key
+    static constexpr int kStat = kRow + ROWS * 8;         // [kWarps][ROWS][2] M and l
+    static constexpr int kBars = kStat + kWarps * ROWS * 8;  // [kWarps][kSlots] mbarriers
+    static constexpr int kBytes = kBars + kWarps * kSlots * 8 + 1024;  // the ring begins at a multiple of 1024
+    // the warps' O meet in the ring; where it is too small for all of D, half of D at a time
+    static constexpr int kParts = kWarps * ROWS * (D + 4) * 4 <= kRing ? 1 : 2;
+    static constexpr int OP = D / kParts + 4;             // floats between rows there
+};
 
 // One tile of q rows of one head against its share of the tokens.  S^T = K.Q^T and O^T = V^T.P^T on
 // mma.m16n8k16: 16 tokens (then 16 dims) x 8 q rows, so a group of 8 or fewer rows wastes at most half of the MMA, and
-// the converted codes of a step serve 8 * NB rows.
+// the converted codes of a step serve 8 * NB rows.  tcgen05's 64 or 128 rows would be mostly padding here.
+//
+// Bound by HBM (4 FLOP per byte and q row).  Each warp runs on its own: its ring of three tiles takes K and V in turn,
+// a tile's place is asked for again as soon as it is read, and no barrier joins the warps before the end of the share.
 template <int FMT, int D, int NB>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) attend_kernel(AttendArgs a) {
-    constexpr int ROWS = 8 * NB;
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NB)) attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap k_map,
+              const __grid_constant__ CUtensorMap v_map) {
+    using L = Layout<D, NB>;
+    constexpr int ROWS = L::ROWS;
     constexpr int CH = D / 16;                // 16-byte chunks of a row of codes
-    constexpr int kSide = kTile * D;          // bytes of one side's tile
-    constexpr int kStage = kSide * 2 + 32;
-    constexpr int QP = 2 * D + 32;            // bytes between q rows: the fragments' 8-byte loads hit all banks
-    extern __shared__ __align__(128) char smem[];
-    char* q_smem = smem + kWarps * kStages * kStage;
-    float* q_scale = reinterpret_cast<float*>(q_smem + ROWS * QP);   // [ROWS] a' = scale * log2(e) / row's power of two
-    int* q_pos = reinterpret_cast<int*>(q_scale + ROWS);             // [ROWS] last key the row sees; -1: none, no row
-    float* stat = reinterpret_cast<float*>(q_pos + ROWS);            // [kWarps][ROWS][2] M, l of the warps
+    extern __shared__ char raw_smem[];
+    char* smem = raw_smem + (1024 - (tc::smem_u32(raw_smem) & 1023)) % 1024;
+    char* q_smem = smem + L::kQ;
+    float* q_scale = reinterpret_cast<float*>(smem + L::kRow);  // [ROWS] a' = scale * log2(e) / row's power of two
+    int* q_pos = reinterpret_cast<int*>(q_scale + ROWS);        // [ROWS] last key the row sees; -1: none, or no row
+    float* stat = reinterpret_cast<float*>(smem + L::kStat);
     __shared__ int64_t sums[kThreads];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t4 = lane & 3;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ int arrived;
 
     int flags = 0;
     const Deal deal = deal_out<ROWS>(a, gridDim.x, sums, &flags);
     if (blockIdx.x == 0 && flags && a.status) atomicOr(a.status, flags);
-    if (deal.total == 0 || blockIdx.x >= deal.ctas) return;
-    int64_t at = deal_start(deal, blockIdx.x);
-    const int64_t stop = deal_start(deal, blockIdx.x + 1);
+    if (deal.total == 0 || blockIdx.x >= deal.ctas) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
+    int64_t at = deal.start(blockIdx.x);
+    const int64_t stop = deal.start(blockIdx.x + 1);
     Place p = find_place<ROWS>(a, deal, sums, at);
 
-    char* ring = smem + warp * kStages * kStage;
-    const uint32_t ring_u32 = smem_addr(ring);
+    const uint32_t ring = tc::smem_u32(smem) + warp * kSlots * L::kSlot;
+    const uint32_t bars = tc::smem_u32(smem + L::kBars) + warp * kSlots * 8;
+    if (lane == 0) {
+        for (int i = 0; i < kSlots; ++i) tc::mbar_init(bars + i * 8, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
     const int pshift = a.cache.page_shift, pmask = a.cache.page_size - 1;
-    const int crow = lane / CH, cchunk = lane % CH;   // this lane's row and chunk of a 16-byte copy
-    constexpr int RPC = 32 / CH;                      // rows per copy instruction
+    uint32_t phases = 0;  // bit i: parity of slot i's next fill
+    bool dead = false;    // a wait gave up: nothing is asked for any more
+    // the fill of a slot, bounded; all lanes see the same outcome
+    const auto wait = [&](int slot) {
+        const uint32_t bar = bars + slot * 8, parity = phases >> slot & 1u;
+        phases ^= 1u << slot;
+        if (__all_sync(~0u, tc::mbar_try_wait(bar, parity)) || dead) return;
+        const uint64_t start = tc::globaltimer();
+        do {
+            if (__all_sync(~0u, tc::mbar_try_wait(bar, parity))) return;
+            dead = __any_sync(~0u, tc::globaltimer() - start > tc::kTimeoutNs);
+        } while (!dead);
+        if (a.status) atomicOr(a.status, PTOWSP_SERVING_TIMEOUT);
+    };
+    // swizzled places of the fragments' 16-byte chunks: rows (lane & 15), chunks c + (lane >> 4)
+    const int frow = lane & 15, fsw = D == 128 ? frow & 7 : (frow >> 1) & 3;
 
     while (at < stop) {
         const int head = static_cast<int>(p.task % a.cache.kv_heads);
@@ -253,57 +407,76 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attend_kernel(AttendArgs
         const int32_t* table = a.page_table + p.r * a.table_stride;
         const int rows = min(ROWS, p.q.nq * a.group - row_base);
 
-        // -- the warp's tiles: tok0 + (warp + 4 i) * 32 --
+        // -- the warp's tiles: first + i * kUnit --
         const int first = tok0 + warp * kTile;
         const int ntiles = tok1 > first ? (tok1 - first + kUnit - 1) / kUnit : 0;
-        // page ids of the two 16-token halves of tile i, lane 0 and 1 (-1: no token there)
+        // page ids of the two 16-token halves of tile i, in lanes 0 and 1 (-1: no token there)
+        const int seen = p.q.seen;
         auto page_of = [&](int i) -> int {
             int id = -1;
             const int tok = first + i * kUnit + lane * 16;
-            if (lane < 2 && i < ntiles && tok < tok1 && tok + 16 > p.q.seen) {
+            if (lane < 2 && tok < tok1 && tok + 16 > seen) {
                 id = table[tok >> pshift];
-                if (id < 0 || id >= a.cache.pages) {
+                if (static_cast<uint32_t>(id) >= a.cache.pages) {
                     id = -1;
                     if (a.status) atomicOr(a.status, PTOWSP_SERVING_PAGE);
                 }
             }
             return id;
         };
-        auto issue = [&](int i, int ids) {
-            if (i < ntiles) {
-                const int tile = first + i * kUnit;
-                const uint32_t dst = ring_u32 + (i % kStages) * kStage;
-#pragma unroll
-                for (int j = 0; j < kTile / RPC; ++j) {
-                    const int row = j * RPC + crow;
-                    const int id = __shfl_sync(~0u, ids, row >> 4);
-                    const int tok = tile + row;
-                    const bool live = id >= 0 && tok < tok1;
-                    const int sw = D == 128 ? (cchunk ^ (row & 7)) : (cchunk ^ ((row >> 1) & 3));
-                    const uint32_t to = dst + row * D + sw * 16;
-                    const int64_t page = live ? id : 0;
-                    const int64_t off = live ? (tok & pmask) : 0;
-                    cp_async16(to, a.cache.k.codes + page * a.cache.k.page_stride + off * a.cache.k.token_stride +
-                                       head * a.cache.k.head_stride + cchunk * 16, live);
-                    cp_async16(to + kSide, a.cache.v.codes + page * a.cache.v.page_stride +
-                                               off * a.cache.v.token_stride + head * a.cache.v.head_stride + cchunk * 16,
-                               live);
-                }
-                const int id = __shfl_sync(~0u, ids, lane & 1);
-                if (lane < 4) {  // k scale of half 0, 1, then v scale of half 0, 1; 0 where there is no page
-                    const float* s = lane < 2 ? a.cache.k.scale : a.cache.v.scale;
-                    cp_async4(dst + 2 * kSide + lane * 4,
-                              s + static_cast<int64_t>(id < 0 ? 0 : id) * a.cache.kv_heads + head, id >= 0);
+        // asks for tile i of one side: one box where the pages hold 32 tokens or more, else one per half
+        auto ask = [&](const CUtensorMap* map, int i, int ids, int slot) {
+            if (i >= ntiles || dead) return;
+            const int id0 = __shfl_sync(~0u, ids, 0), id1 = __shfl_sync(~0u, ids, 1);
+            if (lane == 0) {
+                const int tok = (first + i * kUnit) & pmask;
+                const uint32_t dst = ring + slot * L::kSlot, bar = bars + slot * 8;
+                if (pmask == 15) {
+                    tc::mbar_expect_tx(bar, ((id0 >= 0) + (id1 >= 0)) * (L::kSlot / 2));
+                    if (id0 >= 0) tma_load_page(dst, map, head, 0, id0, bar);
+                    if (id1 >= 0) tma_load_page(dst + L::kSlot / 2, map, head, 0, id1, bar);
+                } else {  // both halves are in one page; the first may lie before the window
+                    const int id = id0 >= 0 ? id0 : id1;
+                    tc::mbar_expect_tx(bar, id >= 0 ? L::kSlot : 0);
+                    if (id >= 0) tma_load_page(dst, map, head, tok, id, bar);
                 }
             }
-            cp_async_commit();
         };
-        int ids = page_of(0);
+        // k scale of half 0 and 1 of a tile, then v's, in lanes 0 .. 3; 0 where there is no page
+        auto scale_of = [&](int ids) -> float {
+            const int id = __shfl_sync(~0u, ids, lane & 1);
+            if (lane >= 4 || id < 0) return 0.f;
+            const float* s = lane < 2 ? a.cache.k.scale : a.cache.v.scale;
+            return s[static_cast<int64_t>(id) * a.cache.kv_heads + head];
+        };
+        // rows of a slot that hold no token become zeros: what stands there could be NaN
+        auto clear = [&](uint32_t slot_addr, int i, float sc0, float sc1) {
+            const int tile = first + i * kUnit;
 #pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) {
-            const int next = page_of(i + 1);
-            issue(i, ids);
-            ids = next;
+            for (int j = 0; j < kTile / 8; ++j) {
+                const int row = j * 8 + (lane >> 2);
+                if (tile + row >= tok1 || !((row < 16 ? sc0 : sc1) > 0.f)) {
+#pragma unroll
+                    for (int c = 0; c < CH / 4; ++c)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(slot_addr + row * D +
+                                                                                     ((lane & 3) + c * 4) * 16),
+                                     "r"(0)
+                                     : "memory");
+                }
+            }
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+        };
+        int ids1, ids2;  // of the tile after the present one, and of the one after that
+        float scales;    // of the present tile
+        {
+            const int ids0 = page_of(0);
+            ids1 = page_of(1);
+            ids2 = page_of(2);
+            ask(&k_map, 0, ids0, 0);
+            ask(&v_map, 0, ids0, 1);
+            ask(&k_map, 1, ids1, 2);
+            scales = scale_of(ids0);
         }
 
         // -- q rows, as f16 times a power of two; one warp per row --
@@ -331,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attend_kernel(AttendArgs
             int e = 0;
             if (m > 0.f && m < INFINITY) e = min(max(14 - (static_cast<int>(__float_as_uint(m) >> 23) - 127), -120), 120);
             const float f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-            __half* to = reinterpret_cast<__half*>(q_smem + row * QP) + lane * (D / 32);
+            __half* to = reinterpret_cast<__half*>(q_smem + row * L::QP) + lane * (D / 32);
 #pragma unroll
             for (int k = 0; k < D / 32; ++k) to[k] = __float2half_rn(x[k] * f);
             if (lane == 0) {
@@ -342,49 +515,52 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attend_kernel(AttendArgs
         __syncthreads();
 
         float qs[NB][2];
-        int pos[NB][2];
-        int min_pos = INT32_MAX, max_pos = -1;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                qs[n][c] = q_scale[n * 8 + 2 * t4 + c];
-                pos[n][c] = q_pos[n * 8 + 2 * t4 + c];
+            for (int c = 0; c < 2; ++c) qs[n][c] = q_scale[n * 8 + 2 * t4 + c];
+        // tiles [plain0, plain0 + plains) need no mask: their 32 tokens exist and every row sees them
+        int plain0 = 0, plains;
+        {
+            const int low = p.q.len - p.q.nq + row_base / a.group;               // the first row's last key
+            const int high = p.q.len - p.q.nq + (row_base + rows - 1) / a.group;  // the last row's
+            const int end = min(tok1, low + 1);
+            plains = end - kTile >= first ? (end - kTile - first) / kUnit + 1 : 0;
+            if (a.window > 0 && high - a.window >= first) {
+                plain0 = (high - a.window - first) / kUnit + 1;
+                plains = max(plains - plain0, 0);
             }
-        for (int i = 0; i < rows; ++i) {  // of the real rows: which tiles need no mask
-            min_pos = min(min_pos, q_pos[i]);
-            max_pos = max(max_pos, q_pos[i]);
         }
-        uint32_t qf[NB <= 2 ? NB : 1][CH][2];
-        if constexpr (NB <= 2) {
+        uint32_t qf[NB == 1 ? CH : 1][2];
+        if constexpr (NB == 1) {
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
-#pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    const uint2 w = *reinterpret_cast<const uint2*>(q_smem + (n * 8 + g) * QP + c * 32 + t4 * 8);
-                    qf[n][c][0] = w.x;
-                    qf[n][c][1] = w.y;
-                }
+            for (int c = 0; c < CH; ++c) {
+                const uint2 w = *reinterpret_cast<const uint2*>(q_smem + g * L::QP + c * 32 + t4 * 8);
+                qf[c][0] = w.x;
+                qf[c][1] = w.y;
+            }
         }
 
         float M[NB][2], l[NB][2], o[NB][CH][4];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            M[n][0] = M[n][1] = -INFINITY;
+            M[n][0] = M[n][1] = kNone;
             l[n][0] = l[n][1] = 0.f;
 #pragma unroll
             for (int c = 0; c < CH; ++c) o[n][c][0] = o[n][c][1] = o[n][c][2] = o[n][c][3] = 0.f;
         }
 
-        for (int i = 0; i < ntiles; ++i) {
-            const int next = page_of(i + kStages);
-            issue(i + kStages - 1, ids);
-            ids = next;
-            cp_async_wait<kStages - 1>();
-            __syncwarp();
-            const int tile = first + i * kUnit;
-            const char* st = ring + (i % kStages) * kStage;
-            const uint32_t st_u32 = ring_u32 + (i % kStages) * kStage;
+        int kslot = 0, vslot = 1;  // of the present tile
+        for (int i = 0; i < ntiles && !dead; ++i) {
+            const int ids3 = page_of(i + 3);
+            const float next_scales = scale_of(ids1);
+            const float sc[4] = {__shfl_sync(~0u, scales, 0), __shfl_sync(~0u, scales, 1), __shfl_sync(~0u, scales, 2),
+                                 __shfl_sync(~0u, scales, 3)};
+            scales = next_scales;
+            // no mask, and no row without a token
+            const bool plain = static_cast<unsigned>(i - plain0) < static_cast<unsigned>(plains) && sc[0] > 0.f && sc[1] > 0.f;
+            wait(kslot);
+            if (!plain) clear(ring + kslot * L::kSlot, i, sc[0], sc[1]);
 
             // S^T: two blocks of 16 tokens
             float s[2][NB][4];
@@ -392,29 +568,29 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attend_kernel(AttendArgs
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int n = 0; n < NB; ++n) s[b][n][0] = s[b][n][1] = s[b][n][2] = s[b][n][3] = 0.f;
+            const uint32_t krow = ring + kslot * L::kSlot + frow * D;
 #pragma unroll
             for (int c = 0; c < CH; c += 2) {
+                const uint32_t at_c = krow + ((c + (lane >> 4)) ^ fsw) * 16;
                 uint32_t qv[NB][2][2];
 #pragma unroll
                 for (int n = 0; n < NB; ++n)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        if constexpr (NB <= 2) {
-                            qv[n][k][0] = qf[n][c + k][0];
-                            qv[n][k][1] = qf[n][c + k][1];
+                        if constexpr (NB == 1) {
+                            qv[n][k][0] = qf[c + k][0];
+                            qv[n][k][1] = qf[c + k][1];
                         } else {
                             const uint2 w =
-                                *reinterpret_cast<const uint2*>(q_smem + (n * 8 + g) * QP + (c + k) * 32 + t4 * 8);
+                                *reinterpret_cast<const uint2*>(q_smem + (n * 8 + g) * L::QP + (c + k) * 32 + t4 * 8);
                             qv[n][k][0] = w.x;
                             qv[n][k][1] = w.y;
                         }
                     }
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
-                    const int row = b * 16 + (lane & 15), ch = c + (lane >> 4);
-                    const int sw = D == 128 ? (ch ^ (row & 7)) : (ch ^ ((row >> 1) & 3));
                     uint32_t w[4];
-                    ldmatrix4(st_u32 + row * D + sw * 16, w);
+                    ldmatrix4(at_c + b * 16 * D, w);
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         uint32_t a0, a1, a2, a3;
@@ -425,47 +601,57 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attend_kernel(AttendArgs
                     }
                 }
             }
+            __syncwarp();
+            ask(&v_map, i + 1, ids1, kslot);  // K's place is free
 
             // exponents t = a' s_k S + log2 s_v
-            const float* sc = reinterpret_cast<const float*>(st + 2 * kSide);
-            const bool plain = tile + kTile <= min(tok1, min_pos + 1) && sc[0] > 0.f && sc[1] > 0.f &&
-                               !(a.window > 0 && tile <= max_pos - a.window);
-            float inv[2];
-            bool grow = false;
+            const float lv[2] = {log2_approx(sc[2]), log2_approx(sc[3])};
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const float ks = sc[b], vs = sc[2 + b];
-                const float lv = log2_approx(vs);
-                inv[b] = 1.f / vs;
+            for (int n = 0; n < NB; ++n)
 #pragma unroll
-                for (int n = 0; n < NB; ++n)
+                for (int c = 0; c < 2; ++c) {
+                    const float f0 = qs[n][c] * sc[0], f1 = qs[n][c] * sc[1];
+                    s[0][n][c] = fmaf(s[0][n][c], f0, lv[0]);
+                    s[0][n][c + 2] = fmaf(s[0][n][c + 2], f0, lv[0]);
+                    s[1][n][c] = fmaf(s[1][n][c], f1, lv[1]);
+                    s[1][n][c + 2] = fmaf(s[1][n][c + 2], f1, lv[1]);
+                }
+            if (!plain) {
+                const int tile = first + i * kUnit;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        float x = fmaf(s[b][n][k], qs[n][k & 1] * ks, lv);
-                        if (!plain) {
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int n = 0; n < NB; ++n)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
                             const int tok = tile + b * 16 + g + (k >> 1) * 8;
-                            const int last = pos[n][k & 1];
-                            const bool seen = ks > 0.f && tok < tok1 && tok <= last &&
-                                              !(a.window > 0 && tok <= last - a.window);
-                            if (!seen) x = -INFINITY;
+                            const int last = q_pos[n * 8 + 2 * t4 + (k & 1)];
+                            const bool see = sc[b] > 0.f && tok < tok1 && tok <= last &&
+                                             !(a.window > 0 && tok <= last - a.window);
+                            if (!see) s[b][n][k] = -INFINITY;
                         }
-                        s[b][n][k] = x;
-                        grow |= x > M[n][k & 1] + 15.f;
-                    }
-                if (!(vs > 0.f)) inv[b] = 0.f;
             }
             // M follows only when a weight would pass 2^15, and then leaves the largest at 2^7
+            float top[NB][2];
+            bool grow = false;
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    top[n][c] = fmaxf(fmaxf(s[0][n][c], s[0][n][c + 2]), fmaxf(s[1][n][c], s[1][n][c + 2]));
+                    grow |= top[n][c] > M[n][c] + 15.f;
+                }
             if (__any_sync(~0u, grow)) {
 #pragma unroll
                 for (int n = 0; n < NB; ++n)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        float m = fmaxf(fmaxf(s[0][n][c], s[0][n][c + 2]), fmaxf(s[1][n][c], s[1][n][c + 2]));
+                        float m = top[n][c];
                         m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
                         m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
                         m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
                         m = fmaxf(m - 7.f, M[n][c]);
-                        const float f = M[n][c] == -INFINITY ? 0.f : exp2_approx(M[n][c] - m);
+                        const float f = exp2_approx(M[n][c] - m);
                         M[n][c] = m;
                         l[n][c] *= f;
 #pragma unroll
@@ -475,28 +661,31 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attend_kernel(AttendArgs
                         }
                     }
             }
+            const float inv[2] = {sc[2] > 0.f ? rcp_approx(sc[2]) : 0.f, sc[3] > 0.f ? rcp_approx(sc[3]) : 0.f};
             uint32_t pb[2][NB][2];
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    const float m0 = M[n][0] == -INFINITY ? 0.f : M[n][0], m1 = M[n][1] == -INFINITY ? 0.f : M[n][1];
-                    const float w0 = exp2_approx(s[b][n][0] - m0), w1 = exp2_approx(s[b][n][1] - m1);
-                    const float w2 = exp2_approx(s[b][n][2] - m0), w3 = exp2_approx(s[b][n][3] - m1);
+                    const float w0 = exp2_approx(s[b][n][0] - M[n][0]), w1 = exp2_approx(s[b][n][1] - M[n][1]);
+                    const float w2 = exp2_approx(s[b][n][2] - M[n][0]), w3 = exp2_approx(s[b][n][3] - M[n][1]);
                     l[n][0] = fmaf(w0 + w2, inv[b], l[n][0]);
                     l[n][1] = fmaf(w1 + w3, inv[b], l[n][1]);
                     pb[b][n][0] = transpose8x8(pack_f16(w0, w1));
                     pb[b][n][1] = transpose8x8(pack_f16(w2, w3));
                 }
+
+            wait(vslot);
+            if (!plain) clear(ring + vslot * L::kSlot, i, sc[0], sc[1]);
             // O^T += V^T.P^T
+            const uint32_t vrow = ring + vslot * L::kSlot + frow * D;
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int c = 0; c < CH; c += 2) {
+                const uint32_t at_c = vrow + ((c + (lane >> 4)) ^ fsw) * 16;
 #pragma unroll
-                for (int c = 0; c < CH; c += 2) {
-                    const int row = b * 16 + (lane & 15), ch = c + (lane >> 4);
-                    const int sw = D == 128 ? (ch ^ (row & 7)) : (ch ^ ((row >> 1) & 3));
+                for (int b = 0; b < 2; ++b) {
                     uint32_t w[4];
-                    ldmatrix4_trans(st_u32 + kSide + row * D + sw * 16, w);
+                    ldmatrix4_trans(at_c + b * 16 * D, w);
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         // bytes (token 2t, dims 2g and 2g + 1), (token 2t + 1, the same): pair the tokens
@@ -507,11 +696,24 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attend_kernel(AttendArgs
                         for (int n = 0; n < NB; ++n) mma16816(o[n][c + k], a0, a1, a2, a3, pb[b][n][0], pb[b][n][1]);
                     }
                 }
+            }
             __syncwarp();
+            ask(&k_map, i + 2, ids2, vslot);  // V's place is free
+            ids1 = ids2;
+            ids2 = ids3;
+            // K of i + 1 stands behind V of i, V of i + 1 where K of i was
+            const int next = vslot == kSlots - 1 ? 0 : vslot + 1;
+            vslot = kslot;
+            kslot = next;
         }
-        cp_async_wait<0>();
 
-        // -- join the warps: O through the ring (every warp is done with it), M and l beside it --
+        if (dead) {  // leave the copies still under way the time to land before their places are used again
+            const uint64_t start = tc::globaltimer();
+            while (tc::globaltimer() - start < tc::kTimeoutNs) {
+            }
+        }
+
+        // -- join the warps: M and l first, then O through the ring, which every warp is done with --
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -526,65 +728,68 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attend_kernel(AttendArgs
                     stat[(warp * ROWS + row) * 2 + 1] = v;
                 }
             }
-        __syncthreads();
-        constexpr int OP = D + 4;  // floats between rows
         float* o_smem = reinterpret_cast<float*>(smem);
+        float* parts = reinterpret_cast<float*>(a.workspace + kArrivals);
+        float* part = parts + (static_cast<int64_t>(blockIdx.x) * 2 + (p.unit > 0 ? 0 : 1)) * partial_floats<D, NB>();
+        constexpr int DP = D / L::kParts;    // dims at a time
+        constexpr int V = DP / 32;           // per lane
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+        for (int h = 0; h < L::kParts; ++h) {
+            __syncthreads();
 #pragma unroll
-            for (int c = 0; c < CH; ++c)
+            for (int n = 0; n < NB; ++n)
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    *reinterpret_cast<float2*>(&o_smem[(warp * ROWS + n * 8 + 2 * t4 + k) * OP + c * 16 + 2 * g]) =
-                        make_float2(o[n][c][k], o[n][c][k + 2]);
-        __syncthreads();
-        float* part = reinterpret_cast<float*>(a.workspace) +
-                      (static_cast<int64_t>(blockIdx.x) * 2 + (p.unit > 0 ? 0 : 1)) * partial_floats<D, NB>();
-        for (int row = warp; row < rows; row += kWarps) {
-            float m = -INFINITY, sum = 0.f;
+                for (int c = 0; c < CH / L::kParts; ++c)
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, stat[(w * ROWS + row) * 2]);
-            float f[kWarps];
+                    for (int k = 0; k < 2; ++k)
+                        *reinterpret_cast<float2*>(&o_smem[(warp * ROWS + n * 8 + 2 * t4 + k) * L::OP + c * 16 + 2 * g]) =
+                            make_float2(o[n][h * (CH / L::kParts) + c][k], o[n][h * (CH / L::kParts) + c][k + 2]);
+            __syncthreads();
+            for (int row = warp; row < rows; row += kWarps) {
+                float m = kNone, sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float mw = stat[(w * ROWS + row) * 2];
-                f[w] = mw == -INFINITY ? 0.f : exp2_approx(mw - m);
-                sum += f[w] * stat[(w * ROWS + row) * 2 + 1];
-            }
-            float x[D / 32];
+                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, stat[(w * ROWS + row) * 2]);
+                float x[V];
 #pragma unroll
-            for (int k = 0; k < D / 32; ++k) x[k] = 0.f;
+                for (int k = 0; k < V; ++k) x[k] = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w)
+                for (int w = 0; w < kWarps; ++w) {
+                    const float f = exp2_approx(stat[(w * ROWS + row) * 2] - m);
+                    sum = fmaf(f, stat[(w * ROWS + row) * 2 + 1], sum);
 #pragma unroll
-                for (int k = 0; k < D / 32; ++k)
-                    x[k] = fmaf(f[w], o_smem[(w * ROWS + row) * OP + lane * (D / 32) + k], x[k]);
-            if (whole) {
-                const int flat = row_base + row;
-                const int64_t tok = p.q.row0 + flat / a.group;
-                const int hq = head * a.group + flat % a.group;
-                const float r = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-                const int64_t off = tok * a.out_token_stride + hq * a.out_head_stride + lane * (D / 32);
-#pragma unroll
-                for (int k = 0; k < D / 32; k += 2) {
-                    if (a.dtype == PTOWSP_F16)
-                        *reinterpret_cast<__half2*>(static_cast<__half*>(a.out) + off + k) =
-                            __floats2half2_rn(x[k] * r, x[k + 1] * r);
-                    else
-                        *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + off + k) =
-                            __floats2bfloat162_rn(x[k] * r, x[k + 1] * r);
+                    for (int k = 0; k < V; ++k) x[k] = fmaf(f, o_smem[(w * ROWS + row) * L::OP + lane * V + k], x[k]);
                 }
-                if (lane == 0 && a.lse)
-                    a.lse[tok * a.heads + hq] = sum > 0.f || sum != sum ? (m + log2f(sum)) * 0.6931471805599453f : -INFINITY;
-            } else {
+                if (whole) {
+                    store_row<V>(a, p.q, head, row_base + row, h * DP + lane * V, x, m, sum, h == 0 && lane == 0);
+                } else {
 #pragma unroll
-                for (int k = 0; k < D / 32; ++k) part[2 * ROWS + row * D + lane * (D / 32) + k] = x[k];
-                if (lane == 0) {
-                    part[row * 2] = m;
-                    part[row * 2 + 1] = sum;
+                    for (int k = 0; k < V; ++k) part[2 * ROWS + row * D + h * DP + lane * V + k] = x[k];
+                    if (h == 0 && lane == 0) {
+                        part[row * 2] = m;
+                        part[row * 2 + 1] = sum;
+                    }
                 }
             }
         }
+        if (!whole) {
+            // the last CTA of the task to come here joins what all of them left
+            const int64_t begin = at - p.unit;
+            const int64_t c0 = deal.owner(begin);
+            const int pieces = static_cast<int>(deal.owner(begin + p.q.units - 1) - c0) + 1;
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                asm volatile("griddepcontrol.wait;" ::: "memory");  // the counters are zero from here on
+                arrived = atomicAdd(reinterpret_cast<int*>(a.workspace) + c0, 1);
+            }
+            __syncthreads();
+            if (arrived == pieces - 1) {
+                __threadfence();
+                join_pieces<D, NB>(a, p.q, head, row_base, rows, parts + (c0 * 2 + 1) * partial_floats<D, NB>(), pieces,
+                                   o_smem);
+            }
+        }
+        tc::fence_proxy_async_smem();  // what was written to the ring here is ordered before the next share's copies
         __syncthreads();
 
         at += take;
@@ -598,88 +803,50 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attend_kernel(AttendArgs
             }
         }
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // on every path: what follows in the stream counts on it
 }
 
-// Joins the partial results of the tasks that the deal cut.  CTA c looks at the cut before CTA c's share and does the
-// work where that is its task's first cut: the pieces are the last one of CTA c - 1 and the first ones of the CTAs
-// from c to the task's end.  One warp per row, its lanes over the dims, warps over the rows.
-template <int D, int NB>
-__global__ void __launch_bounds__(kThreads) join_kernel(AttendArgs a, int ctas) {
-    constexpr int ROWS = 8 * NB;
-    __shared__ int64_t sums[kThreads];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const Deal deal = deal_out<ROWS>(a, ctas, sums, nullptr);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t c = blockIdx.x + 1;
-    if (c >= deal.ctas) return;
-    const int64_t at = deal_start(deal, c);
-    const Place p = find_place<ROWS>(a, deal, sums, at);
-    if (p.unit == 0) return;  // a cut between tasks
-    const int64_t begin = at - p.unit, end = begin + p.q.units;
-    if (deal_start(deal, c - 1) > begin) return;  // an earlier cut of this task has it
-    int64_t last = c;
-    while (last + 1 < deal.ctas && deal_start(deal, last + 1) < end) ++last;
-    const int pieces = static_cast<int>(last - c) + 2;
-    const int head = static_cast<int>(p.task % a.cache.kv_heads);
-    const int row_base = static_cast<int>(p.task / a.cache.kv_heads) * ROWS;
-    const int rows = min(ROWS, p.q.nq * a.group - row_base);
-    const float* ws = reinterpret_cast<const float*>(a.workspace);
-    auto piece = [&](int i) {
-        return ws + (i == 0 ? (c - 1) * 2 + 1 : (c + i - 1) * 2) * static_cast<int64_t>(partial_floats<D, NB>());
-    };
-    for (int row = blockIdx.y * kWarps + warp; row < rows; row += gridDim.y * kWarps) {
-        float m = -INFINITY;
-        for (int i = lane; i < pieces; i += 32) m = fmaxf(m, __ldcg(piece(i) + row * 2));
-#pragma unroll
-        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-        float x[D / 32], sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k) x[k] = 0.f;
-#pragma unroll 8
-        for (int i = 0; i < pieces; ++i) {
-            const float* q = piece(i);
-            const float mi = __ldcg(q + row * 2), li = __ldcg(q + row * 2 + 1);
-            const float f = mi == -INFINITY ? 0.f : exp2_approx(mi - m);
-            sum = fmaf(f, li, sum);
-#pragma unroll
-            for (int k = 0; k < D / 32; ++k)
-                x[k] = fmaf(f, __ldcg(q + 2 * ROWS + row * D + lane * (D / 32) + k), x[k]);
-        }
-        const int flat = row_base + row;
-        const int64_t tok = p.q.row0 + flat / a.group;
-        const int hq = head * a.group + flat % a.group;
-        const float r = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-        const int64_t off = tok * a.out_token_stride + hq * a.out_head_stride + lane * (D / 32);
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-            if (a.dtype == PTOWSP_F16) static_cast<__half*>(a.out)[off + k] = __float2half_rn(x[k] * r);
-            else static_cast<__nv_bfloat16*>(a.out)[off + k] = __float2bfloat16_rn(x[k] * r);
-        }
-        if (lane == 0 && a.lse)
-            a.lse[tok * a.heads + hq] = sum > 0.f || sum != sum ? (m + log2f(sum)) * 0.6931471805599453f : -INFINITY;
-    }
+// The codes as a tensor [pages][page_size][heads][D] whose box is one head's D bytes of up to 32 tokens of a page.
+bool page_map(CUtensorMap* m, const Kv8& c, const Kv8Side& side) {
+    const uint64_t dims[4] = {static_cast<uint64_t>(c.head_dim), static_cast<uint64_t>(c.kv_heads),
+                              static_cast<uint64_t>(c.page_size), static_cast<uint64_t>(c.pages)};
+    // a dimension of one element has no stride that matters
+    const uint64_t strides[3] = {c.kv_heads > 1 ? static_cast<uint64_t>(side.head_stride) : dims[0],
+                                 static_cast<uint64_t>(side.token_stride),
+                                 c.pages > 1 ? static_cast<uint64_t>(side.page_stride) : dims[0]};
+    const uint32_t box[4] = {static_cast<uint32_t>(c.head_dim), 1, c.page_size < 32 ? 16u : 32u, 1};
+    return tc::make_map_u8_4d(m, side.codes, dims, strides, box);
+}
+
+// Zeroes the arrival counters.  The attention starts beside it and waits for it before its first arrival.
+__global__ void clear_arrivals(int* counts, int n) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    for (int i = threadIdx.x; i < n; i += blockDim.x) counts[i] = 0;
 }
 
 template <int FMT, int D, int NB>
 cudaError_t launch_rows(const AttendArgs& a, int sms, cudaStream_t s) {
-    constexpr int smem = attend_smem<D, NB>();
-    cudaError_t e = cudaFuncSetAttribute(attend_kernel<FMT, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    constexpr int smem = Layout<D, NB>::kBytes;
+    static SmemOptIn opt_in;
+    cudaError_t e = opt_in.once(reinterpret_cast<const void*>(attend_kernel<FMT, D, NB>), smem);
     if (e != cudaSuccess) return e;
-    const int ctas = sms * kCtasPerSm;
-    attend_kernel<FMT, D, NB><<<ctas, kThreads, smem, s>>>(a);
+    const int ctas = sms * ctas_per_sm(NB);
+    CUtensorMap k_map, v_map;
+    if (!page_map(&k_map, a.cache, a.cache.k) || !page_map(&v_map, a.cache, a.cache.v)) return cudaErrorInvalidValue;
+    clear_arrivals<<<1, 256, 0, s>>>(reinterpret_cast<int*>(a.workspace), ctas);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    // the join starts while the last CTAs finish; it waits for them before it reads
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas - 1, 2 * NB);
+    cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, join_kernel<D, NB>, a, ctas);
+    return cudaLaunchKernelEx(&cfg, attend_kernel<FMT, D, NB>, a, k_map, v_map);
 }
 
 template <int FMT, int D>
@@ -695,7 +862,7 @@ cudaError_t launch_d(const AttendArgs& a, int sms, cudaStream_t s) {
 size_t attend_workspace_bytes(const AttendArgs& a, int sms) {
     const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
     const int nb = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-    return static_cast<size_t>(sms) * kCtasPerSm * 2 * (8 * nb) * (a.cache.head_dim + 2) * sizeof(float);
+    return kArrivals + static_cast<size_t>(sms) * ctas_per_sm(nb) * 2 * (8 * nb) * (a.cache.head_dim + 2) * sizeof(float);
 }
 
 cudaError_t launch_attend(const AttendArgs& a, int sms, cudaStream_t s) {

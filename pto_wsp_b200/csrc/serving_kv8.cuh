@@ -11,20 +11,14 @@
 
 namespace ptowsp::dev {
 
-// Two e4m3 codes (low half of w) as two f16: exact, f16 has every e4m3 value.
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w) {
-    uint32_t r;
-    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(w));
-    return r;
-}
-
 // Bytes 0, 1 -> lo and bytes 2, 3 -> hi as f16 pairs, exactly.  int8: the byte with its sign flipped is the low
 // mantissa byte of 1024 + (code + 128), from which 1152 is taken.
 template <int FMT>
 __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
     if (FMT == PTOWSP_KV8_E4M3) {
-        lo = e4m3x2_f16x2(w);
-        hi = e4m3x2_f16x2(w >> 16);
+        asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
     } else {
         w ^= 0x80808080u;
         lo = __byte_perm(w, 0x64646464u, 0x4140);

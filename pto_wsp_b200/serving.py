@@ -18,6 +18,7 @@ with torch's allocator on the current stream, and keep nothing.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import NamedTuple
 
 import torch
@@ -68,6 +69,16 @@ class _Sample(C.Structure):
                 ("token", _P), ("logprob", _P)]
 
 
+def _packer(cls):
+    """The struct's C layout as a bytes packer: filling a ctypes structure field by field takes twice as long."""
+    codes = {_P: "P", _I64: "q", _I32: "i", _F32: "f", C.c_size_t: "N"}
+    fmt = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_))
+    assert fmt.size == C.sizeof(cls)
+    return fmt.pack
+
+
+_pack_reserve, _pack_cache, _pack_append, _pack_attention, _pack_sample = map(
+    _packer, (_Reserve, _Cache, _Append, _Attention, _Sample))
 _lib = None
 
 
@@ -84,14 +95,13 @@ def _library():
     return _lib
 
 
-def _call(fn, device, *structs):
-    """Call a C entry on `device` and its current stream."""
-    args = [C.addressof(s) for s in structs]
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+def _call(fn, index, *structs):
+    """Call a C entry on device `index` and its current stream (read as torch.cuda.current_stream reads it)."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*structs, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*structs, torch._C._cuda_getCurrentRawStream(index))
     if rc != PTOWSP_OK:
         raise PtoWspCudaError(rc, (_library().ptowsp_cuda_last_error() or b"").decode())
 
@@ -101,33 +111,30 @@ def _need(cond, text):
         raise ValueError(text)
 
 
-def _vector(t, name, dtype, n, device):
-    """A contiguous 1-D tensor of n elements, as its address."""
-    if t.dtype != dtype:
+def _cuda_index(t, name):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    return t.get_device()
+
+
+def _vector(t, name, dtype, n, index):
+    """A contiguous 1-D tensor of n elements, as its address; 0 for None."""
+    if t is None:
+        return 0
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype} (got {t.dtype})")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous, of {n} elements (got {tuple(t.shape)})")
+    if t.shape != (n,) or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError(f"{name} must be contiguous, of {n} elements, on cuda:{index} (got {tuple(t.shape)} on {t.device})")
     return t.data_ptr()
 
 
-def _status(t, device):
-    return None if t is None else _vector(t, "status", torch.int32, 1, device)
-
-
-def _cuda_device(t, name):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise TypeError(f"{name} must be a CUDA tensor")
-    return t.device
-
-
-def _table(t, requests, device):
-    if t.dtype != torch.int32:
+def _table(t, requests, index):
+    if t.dtype is not torch.int32:
         raise TypeError(f"page_table must be torch.int32 (got {t.dtype})")
-    if t.device != device or t.dim() != 2 or t.shape[0] != requests or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"page_table must be [{requests}, max_pages] on {device}, its rows contiguous")
-    return t.data_ptr(), t.stride(0) if requests > 1 else max(t.stride(0), t.shape[1]), t.shape[1]
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != requests or t.get_device() != index or (shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"page_table must be [{requests}, max_pages] on cuda:{index}, its rows contiguous")
+    return t.data_ptr(), t.stride(0) if requests > 1 else shape[1], shape[1]
 
 
 def check_status(status: torch.Tensor) -> None:
@@ -157,48 +164,41 @@ def reserve_pages(page_table, kv_len, new_tokens, free_ring, free_state, *, page
     ``new_tokens`` are int32 [requests], ``free_state`` int64 [2] (head, tail: the ring holds the free page ids at
     head .. tail - 1 modulo n).  ``max_tokens``: length of the token list, at least the sum of the new tokens.
     A request that finds no room is refused whole: its length stays and its slots are -1."""
-    device = _cuda_device(page_table, "page_table")
-    _need(kv_len.dim() == 1, "kv_len must be [requests]")
-    requests = kv_len.shape[0]
-    table, stride, max_pages = _table(page_table, requests, device)
+    index = _cuda_index(page_table, "page_table")
+    i32, i64 = torch.int32, torch.int64
+    requests, cap = kv_len.shape[0], free_ring.shape[0]
+    table, stride, max_pages = _table(page_table, requests, index)
     _need(max_tokens >= 0, "max_tokens must not be negative")
-    _need(free_ring.dim() == 1, "free_ring must be one-dimensional")
-    i32 = torch.int32
-    a = _Reserve(table, stride, max_pages, page_size, requests, 0, _vector(kv_len, "kv_len", i32, requests, device),
-                 _vector(new_tokens, "new_tokens", i32, requests, device),
-                 _vector(free_ring, "free_ring", i32, free_ring.shape[0], device), free_ring.shape[0],
-                 _vector(free_state, "free_state", torch.int64, 2, device))
-    # one allocation for the int64 results and one for the int32 ones
-    longs = torch.empty(max_tokens + 2, dtype=torch.int64, device=device)
-    ints = torch.empty(max_tokens + 2 * requests + 1, dtype=i32, device=device)
-    granted = torch.empty(requests, dtype=torch.bool, device=device)
-    free_out, slots = longs[:2], longs[2:]
-    q_start, len_out, positions = ints.split((requests + 1, requests, max_tokens))
-    a.slots, a.positions, a.max_tokens = slots.data_ptr(), positions.data_ptr(), max_tokens
-    a.q_start, a.kv_len_out, a.free_state_out = q_start.data_ptr(), len_out.data_ptr(), free_out.data_ptr()
-    a.granted, a.status = granted.data_ptr(), _status(status, device)
-    _call(_library().ptowsp_cuda_reserve_pages, device, a)
-    return PageStep(slots, positions, q_start, len_out, free_out, granted)
+    len_in, state_in = _vector(kv_len, "kv_len", i32, requests, index), _vector(free_state, "free_state", i64, 2, index)
+    len_out, state_out = torch.empty_like(kv_len), torch.empty_like(free_state)
+    q_start, positions, slots = kv_len.new_empty(requests + 1), kv_len.new_empty(max_tokens), free_state.new_empty(max_tokens)
+    granted = torch.empty_like(kv_len, dtype=torch.bool)
+    _call(_library().ptowsp_cuda_reserve_pages, index, _pack_reserve(
+        table, stride, max_pages, page_size, requests, 0, len_in,
+        _vector(new_tokens, "new_tokens", i32, requests, index), _vector(free_ring, "free_ring", i32, cap, index), cap,
+        state_in, slots.data_ptr(), positions.data_ptr(), max_tokens, q_start.data_ptr(), len_out.data_ptr(),
+        state_out.data_ptr(), granted.data_ptr(), _vector(status, "status", i32, 1, index)))
+    return PageStep(slots, positions, q_start, len_out, state_out, granted)
 
 
 def _cache(k_cache, v_cache, k_scale, v_scale):
-    device = _cuda_device(k_cache, "k_cache")
+    """Checks a cache; its device, the packed struct, heads and head_dim."""
+    index = _cuda_index(k_cache, "k_cache")
     fmt = _FORMATS.get(k_cache.dtype)
-    if fmt is None or v_cache.dtype != k_cache.dtype:
+    if fmt is None or v_cache.dtype is not k_cache.dtype:
         raise TypeError(f"k_cache and v_cache must both be float8_e4m3fn or int8 (got {k_cache.dtype}, {v_cache.dtype})")
-    shape = k_cache.shape
-    _need(len(shape) == 4 and v_cache.shape == shape, "k_cache and v_cache must be [pages, page_size, heads, head_dim]")
-    ks, vs = k_cache.stride(), v_cache.stride()
-    _need(ks[3] == 1 and vs[3] == 1, "the cache's last dimension must be contiguous")
+    shape, ks, vs = k_cache.shape, k_cache.stride(), v_cache.stride()
+    if len(shape) != 4 or v_cache.shape != shape or ks[3] != 1 or vs[3] != 1 or v_cache.get_device() != index:
+        raise ValueError(f"k_cache and v_cache must be [pages, page_size, heads, head_dim] on cuda:{index}, the last "
+                         f"dimension contiguous (got {tuple(shape)}, {tuple(v_cache.shape)})")
     pages, page, heads, dim = shape
-    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        if t.dtype != torch.float32:
-            raise TypeError(f"{name} must be torch.float32 (got {t.dtype})")
-        _need(t.shape == (pages, heads) and t.is_contiguous() and t.device == device,
-              f"{name} must be contiguous [{pages}, {heads}] on {device}")
-    _need(v_cache.device == device, f"v_cache must be on {device}")
-    return device, _Cache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ks[0], ks[1],
-                          ks[2], vs[0], vs[1], vs[2], pages, page, heads, dim, fmt)
+    for t in (k_scale, v_scale):
+        if t.dtype is not torch.float32:
+            raise TypeError(f"k_scale and v_scale must be torch.float32 (got {t.dtype})")
+        if t.shape != (pages, heads) or not t.is_contiguous() or t.get_device() != index:
+            raise ValueError(f"k_scale and v_scale must be contiguous [{pages}, {heads}] on cuda:{index}")
+    return index, _pack_cache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ks[0],
+                              ks[1], ks[2], vs[0], vs[1], vs[2], pages, page, heads, dim, fmt), heads, dim
 
 
 def append_kv8(k, v, slots, k_cache, v_cache, k_scale, v_scale, *, status=None) -> None:
@@ -208,19 +208,18 @@ def append_kv8(k, v, slots, k_cache, v_cache, k_scale, v_scale, *, status=None) 
     The cache, codes [pages, page_size, heads, head_dim] in float8_e4m3fn or int8 with any page, token and head order,
     has one float32 scale per page and head.  A page's scale grows with its tokens, and its earlier codes are then
     rounded again; writing a page's first token begins its scale anew."""
-    device, cache = _cache(k_cache, v_cache, k_scale, v_scale)
+    index, cache, heads, dim = _cache(k_cache, v_cache, k_scale, v_scale)
     tokens = k.shape[0]
-    size = (tokens, cache.num_kv_heads, cache.head_dim)
     dtype = _DTYPES.get(k.dtype)
-    if dtype is None or v.dtype != k.dtype:
+    if dtype is None or v.dtype is not k.dtype:
         raise TypeError(f"k and v must both be float32, float16 or bfloat16 (got {k.dtype}, {v.dtype})")
-    ks, vs = k.stride(), v.stride()
-    _need(k.shape == size and v.shape == size, f"k and v must be {size} (got {tuple(k.shape)}, {tuple(v.shape)})")
-    _need(k.device == device and v.device == device, f"k and v must be on {device}")
-    _need(ks[2] == 1 and vs[2] == 1, "the last dimension of k and v must be contiguous")
-    a = _Append(k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
-                _vector(slots, "slots", torch.int64, tokens, device), tokens, dtype, 0, _status(status, device))
-    _call(_library().ptowsp_cuda_kv8_append, device, cache, a)
+    size, ks, vs = (tokens, heads, dim), k.stride(), v.stride()
+    if k.shape != size or v.shape != size or ks[2] != 1 or vs[2] != 1 or k.get_device() != index or v.get_device() != index:
+        raise ValueError(f"k and v must be {size} on cuda:{index}, the last dimension contiguous (got {tuple(k.shape)}, "
+                         f"{tuple(v.shape)})")
+    _call(_library().ptowsp_cuda_kv8_append, index, cache, _pack_append(
+        k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], _vector(slots, "slots", torch.int64, tokens, index),
+        tokens, dtype, 0, _vector(status, "status", torch.int32, 1, index)))
 
 
 def attend_kv8(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_len, *, q_start=None, max_q: int = 1, scale=None,
@@ -232,37 +231,38 @@ def attend_kv8(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_len, *, q_s
     the cached tokens, the new ones included, whose pages stand in ``page_table`` int32 [requests, max_pages].
     ``scale`` of the scores: 1 / sqrt(head_dim) unless given; ``window`` > 0: a row sees its own token and the
     window - 1 before it.  Returns out like q, and with ``return_lse`` also float32 [tokens, heads]."""
-    device, cache = _cache(k_cache, v_cache, k_scale, v_scale)
+    index, cache, _, dim = _cache(k_cache, v_cache, k_scale, v_scale)
     dtype = _DTYPES.get(q.dtype)
     if not dtype:
         raise TypeError(f"q must be float16 or bfloat16 (got {q.dtype})")
-    _need(q.dim() == 3 and q.shape[2] == cache.head_dim and q.device == device,
-          f"q must be [tokens, heads, {cache.head_dim}] on {device}")
-    tokens, heads = q.shape[0], q.shape[1]
+    shape, qs = q.shape, q.stride()
+    if len(shape) != 3 or shape[2] != dim or qs[2] != 1 or q.get_device() != index:
+        raise ValueError(f"q must be [tokens, heads, {dim}] on cuda:{index}, the last dimension contiguous (got {tuple(shape)})")
+    tokens, heads, _ = shape
     if out is None:
-        out = torch.empty((tokens, heads, cache.head_dim), dtype=q.dtype, device=device)
+        out, os = q.new_empty(shape), (heads * dim, dim, 1)
     else:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == device, "out must be like q")
-    qs, os = q.stride(), out.stride()
-    _need(qs[2] == 1 and os[2] == 1, "the last dimension of q and out must be contiguous")
-    _need(kv_len.dim() == 1, "kv_len must be [requests]")
+        os = out.stride()
+        if out.shape != shape or out.dtype is not q.dtype or out.get_device() != index or os[2] != 1:
+            raise ValueError("out must be like q")
+    i32 = torch.int32
     requests = kv_len.shape[0]
-    table, stride, max_pages = _table(page_table, requests, device)
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
-    a = _Attention(q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, qs[0], qs[1], os[0], os[1],
-                   table, stride, _vector(kv_len, "kv_len", torch.int32, requests, device),
-                   None if q_start is None else _vector(q_start, "q_start", torch.int32, requests + 1, device), tokens,
-                   max_pages, requests, heads, max_q, window, dtype,
-                   cache.head_dim ** -0.5 if scale is None else scale, 0, None, 0, _status(status, device))
+    table, stride, max_pages = _table(page_table, requests, index)
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
+    # all but the workspace, its size and the status
+    head = (q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, qs[0], qs[1], os[0], os[1], table, stride,
+            _vector(kv_len, "kv_len", i32, requests, index), _vector(q_start, "q_start", i32, requests + 1, index), tokens,
+            max_pages, requests, heads, max_q, window, dtype, dim ** -0.5 if scale is None else scale, 0)
     lib = _library()
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            nbytes = lib.ptowsp_cuda_kv8_attention_workspace(C.addressof(cache), C.addressof(a))
+    a = _pack_attention(*head, 0, 0, 0)
+    if index == torch._C._cuda_getDevice():
+        nbytes = lib.ptowsp_cuda_kv8_attention_workspace(cache, a)
     else:
-        nbytes = lib.ptowsp_cuda_kv8_attention_workspace(C.addressof(cache), C.addressof(a))
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), nbytes
-    _call(lib.ptowsp_cuda_kv8_attention, device, cache, a)
+        with torch.cuda.device(index):
+            nbytes = lib.ptowsp_cuda_kv8_attention_workspace(cache, a)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _call(lib.ptowsp_cuda_kv8_attention, index, cache,
+          _pack_attention(*head, workspace.data_ptr(), nbytes, _vector(status, "status", i32, 1, index)))
     return (out, lse) if return_lse else out
 
 
@@ -274,20 +274,20 @@ def sample_tokens(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=
     ``top_p`` float32 (1: all), ``min_p`` float32 (0: all), applied in the order temperature, top-k, min-p, top-p.
     Returns the tokens, int32 [rows] (-1 where every logit is -inf or NaN), and the logarithm of each one's
     probability among what the settings left, float32 [rows]."""
-    device = _cuda_device(logits, "logits")
+    index = _cuda_index(logits, "logits")
     dtype = _DTYPES.get(logits.dtype)
     if dtype is None:
         raise TypeError(f"logits must be float32, float16 or bfloat16 (got {logits.dtype})")
-    _need(logits.dim() == 2 and (logits.shape[1] < 2 or logits.stride(1) == 1), "logits must be [rows, vocab], rows contiguous")
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be [rows, vocab], its rows contiguous")
     rows, vocab = logits.shape
     f32 = torch.float32
-    token = torch.empty(rows, dtype=torch.int32, device=device)
-    logprob = torch.empty(rows, dtype=f32, device=device)
-    a = _Sample(logits.data_ptr(), logits.stride(0), rows, vocab, dtype, 0, _vector(u, "u", f32, rows, device),
-                None if temperature is None else _vector(temperature, "temperature", f32, rows, device),
-                None if top_k is None else _vector(top_k, "top_k", torch.int32, rows, device),
-                None if top_p is None else _vector(top_p, "top_p", f32, rows, device),
-                None if min_p is None else _vector(min_p, "min_p", f32, rows, device), token.data_ptr(),
-                logprob.data_ptr())
-    _call(_library().ptowsp_cuda_sample_tokens, device, a)
+    at_u = _vector(u, "u", f32, rows, index)
+    logprob = torch.empty_like(u)
+    token = torch.empty_like(u, dtype=torch.int32)
+    _call(_library().ptowsp_cuda_sample_tokens, index, _pack_sample(
+        logits.data_ptr(), logits.stride(0), rows, vocab, dtype, 0, at_u,
+        _vector(temperature, "temperature", f32, rows, index), _vector(top_k, "top_k", torch.int32, rows, index),
+        _vector(top_p, "top_p", f32, rows, index), _vector(min_p, "min_p", f32, rows, index), token.data_ptr(),
+        logprob.data_ptr()))
     return token, logprob
