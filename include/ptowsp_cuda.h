@@ -364,7 +364,7 @@ PTOWSP_API int ptowsp_cuda_kv8_attention(const ptowsp_kv8_cache* cache, const pt
 PTOWSP_API size_t ptowsp_cuda_kv8_attention_workspace(const ptowsp_kv8_cache* cache,
                                                       const ptowsp_kv8_attention_args* args);
 
-/* One token per row of logits [rows][vocab] (f32, f16 or bf16; rows `row_stride` elements apart), from one uniform
+/* One token per row of logits [rows][vocab] (f32, f16 or bf16; rows `row_stride` elements apart; vocab up to 393216), from one uniform
  * random number u[row] in [0, 1) each.  With the row's largest logit M, w_i = exp((x_i - M) / temperature), taken as a
  * whole number of 2^-40 (so its sums do not depend on their order).  Ordered by falling logit, ties by rising index,
  * the candidates are cut to the first top_k, to w_i >= min_p, and then to the shortest prefix that holds top_p of what

@@ -97,6 +97,8 @@ struct AttendArgs {
 size_t attend_workspace_bytes(const AttendArgs& a, int sms);
 cudaError_t launch_attend(const AttendArgs& a, int sms, cudaStream_t s);
 
+constexpr int kSampleMaxSmem = 224 << 10;  // of a CTA: its slice of the row, histograms and lists
+constexpr int kSampleMaxVocab = 393216;    // eight slices of 192 KB of f32
 struct SampleArgs {
     const void* logits;
     int64_t row_stride;

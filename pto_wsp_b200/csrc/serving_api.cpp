@@ -211,7 +211,8 @@ int ptowsp_cuda_sample_tokens(const ptowsp_sample_args* g, void* stream) {
     const char* what = "sample_tokens";
     if (!g) return fail(PTOWSP_ERR_ARG, "%s: null argument", what);
     if (g->rows < 0 || g->vocab < 1) return fail(PTOWSP_ERR_ARG, "%s: rows must be >= 0 and vocab >= 1", what);
-    if (g->vocab > (1 << 22)) return fail(PTOWSP_ERR_LIMIT, "%s: vocab must be at most 2^22 (got %d)", what, g->vocab);
+    if (g->vocab > kSampleMaxVocab)
+        return fail(PTOWSP_ERR_LIMIT, "%s: vocab must be at most %d (got %d)", what, kSampleMaxVocab, g->vocab);
     if (g->dtype != PTOWSP_F32 && g->dtype != PTOWSP_F16 && g->dtype != PTOWSP_BF16)
         return fail(PTOWSP_ERR_UNSUPPORTED, "%s: logits must be f32, f16 or bf16", what);
     if (g->rows == 0) return PTOWSP_OK;
