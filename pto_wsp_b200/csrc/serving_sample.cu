@@ -53,9 +53,19 @@ struct Element {
     int64_t w;
 };
 
+// w * 2^40 without its fraction, for 0 <= w <= 1: the 24 significant bits, moved (the conversion instruction for 64-bit
+// integers has a sixteenth of this rate).
+__device__ __forceinline__ int64_t whole_of(float w) {
+    const uint32_t u = __float_as_uint(w);
+    const int e = static_cast<int>(u >> 23) - 110;  // w = m * 2^(e - 40)
+    const uint64_t m = (u & 0x7fffffu) | 0x800000u;
+    return e >= 0 ? static_cast<int64_t>(m << e) : e > -24 ? static_cast<int64_t>(static_cast<uint32_t>(m) >> -e) : 0;
+}
+
 // What a CTA shows to the others of its cluster.  Each step has a place of its own, written once between two barriers.
 struct Board {
-    uint64_t best;
+    float top;
+    int index;
     int64_t mass[3];
     int count[3];
     uint64_t low, high;
@@ -114,8 +124,10 @@ struct Row {
     SharedCut* cuts;
     int first, n;          // its first index and its length
     float top, t, min_p;
+    float inv;             // RN(1 / t) where the quotient may be made from it, else 0
     float low;             // what is below is no candidate
     uint64_t cut = 0;      // candidates are at or above
+    bool raised = false;   // `low` leaves out elements that have a weight
 
     __device__ void sync() const {
         if constexpr (CL > 1) cg::this_cluster().sync();
@@ -126,19 +138,28 @@ struct Row {
         if constexpr (CL > 1) return cg::this_cluster().map_shared_rank(const_cast<V*>(p), rank);
         else return p;
     }
-    __device__ float distance(float v) const { return __fdiv_rn(v - top, t); }
+    // (v - top) / t, correctly rounded: Markstein's theorem gives that from RN(1 / t) by one fused correction of a
+    // quotient that is within an ulp, which the first correction makes it.  For t within 2^-40 .. 2^40 no step
+    // underflows, but where the quotient is so small that its exponential is 1.
+    __device__ float distance(float v) const {
+        const float a = v - top;
+        float q = a * inv;
+        q = fmaf(fmaf(-q, t, a), inv, q);
+        return fmaf(fmaf(-q, t, a), inv, q);
+    }
+    __device__ float any_distance(float v) const { return inv != 0.f ? distance(v) : __fdiv_rn(v - top, t); }
     // the candidate's weight, 0: none.  `v` is at or above `low`.
     __device__ int64_t weigh(float v, int i) const {
         float w = 1.f;
         if (v != top) {
-            w = expf(distance(v));
+            w = expf(any_distance(v));
             if (!(w >= min_p) || !(v > -INFINITY)) return 0;
         }
         if (CUTS && composite(v, first + i) < cut) return 0;
-        return static_cast<int64_t>(w * 1099511627776.f);
+        return whole_of(w);
     }
     __device__ int bin_of(float v) const {
-        const float b = -distance(v) * kBinsPerUnit;
+        const float b = -any_distance(v) * kBinsPerUnit;
         return b < kBins ? static_cast<int>(b) : kBins - 1;  // NaN (an infinite row's rest) is in the last bin
     }
 
@@ -154,15 +175,35 @@ struct Row {
     // Masses of the warps' regions, and the cluster's mass and count of candidates.
     __device__ void weigh_regions(int step, int64_t* mass, int* count) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        const int size = region_size();
+        const int size = region_size(), end = min(n, (warp + 1) * size);
         int64_t m = 0;
         int k = 0;
-        for (int i = warp * size + lane; i < min(n, (warp + 1) * size); i += 32) {
-            const float v = as_float(x[i]);
-            if (!(v < low) && v == v) {
-                const int64_t w = weigh(v, i);
-                m += w;
-                k += w > 0;
+        if (inv != 0.f && top < INFINITY && !(CUTS && (cut || raised))) {
+            // The whole row, with no branch: the weight of -inf or NaN comes out as NaN and is none, what is out of reach
+            // has no whole part.  w * 2^40 is taken in two parts of 20 bits: adding 2^23 with rounding towards zero
+            // leaves floor(w * 2^20) in the low bits, and the rest of the product is exact.  A thread's parts sum to
+            // less than 2^32: it has some 200 elements at most, and a part is at most 2^20.
+            uint32_t hi = 0, lo = 0;
+#pragma unroll 4
+            for (int i = warp * size + lane; i < end; i += 32) {
+                float w = expf(distance(as_float(x[i])));
+                w = w >= min_p ? w : 0.f;
+                const float h = __fmaf_rz(w, 1048576.f, 8388608.f);
+                const float rest = fmaf(w, 1048576.f, 8388608.f - h);
+                const float l = __fmaf_rz(rest, 1048576.f, 8388608.f);
+                hi += __float_as_uint(h) - 0x4b000000u;
+                lo += __float_as_uint(l) - 0x4b000000u;
+                if (CUTS) k += w >= 9.094947e-13f;
+            }
+            m = (static_cast<int64_t>(hi) << 20) + lo;
+        } else {
+            for (int i = warp * size + lane; i < end; i += 32) {
+                const float v = as_float(x[i]);
+                if (!(v < low) && v == v) {
+                    const int64_t w = weigh(v, i);
+                    m += w;
+                    k += w > 0;
+                }
             }
         }
 #pragma unroll
@@ -187,6 +228,7 @@ struct Row {
         sync();
         *mass = 0;
         *count = 0;
+#pragma unroll
         for (int r = 0; r < CL; ++r) {
             const Board* b = of(&sh.board, r);
             *mass += b->mass[step];
@@ -195,11 +237,10 @@ struct Row {
     }
     __device__ int region_size() const { return ((n + kWarps - 1) / kWarps + 31) & ~31; }
 
-    // Gathers the cluster's lists (at most kList elements in all) and finds the element at which the running measure,
-    // from `before` on, reaches `target`: sets `cut` to it and returns the measure with it.
-    template <bool MASS>
-    __device__ int64_t rank_list(int64_t before, int64_t target, int total) {
+    // Gathers the cluster's lists, at most kList elements in all.
+    __device__ void gather() {
         int at = 0;
+#pragma unroll
         for (int r = 0; r < CL; ++r) {
             const int k = of(&sh.board, r)->listed;
             const Element* from = of(cuts->list, r);
@@ -207,6 +248,12 @@ struct Row {
             at += k;
         }
         __syncthreads();
+    }
+
+    // The element of the gathered list at which the running measure, from `before` on, reaches `target`: sets `cut`.
+    template <bool MASS>
+    __device__ void rank_list(int64_t before, int64_t target, int total) {
+        gather();
         // two threads per element, each against half of the list
         const int e = threadIdx.x >> 1, half = threadIdx.x & 1;
         const Element me = e < total ? cuts->all[e] : Element{0, 0};
@@ -218,13 +265,62 @@ struct Row {
         m += __shfl_xor_sync(~0u, m, 1);
         m += before;
         const int64_t with = m + (MASS ? me.w : 1);
-        if (e < total && half == 0 && m < target && with >= target) {
-            sh.cut = me.c;
-            sh.cut_mass = with;
-        }
+        if (e < total && half == 0 && m < target && with >= target) sh.cut = me.c;
         __syncthreads();
         cut = sh.cut;
-        return sh.cut_mass;
+    }
+
+    // All that is left to do where the lists hold every candidate: the first k of them (0: all), of these the shortest
+    // prefix of mass `limit` (0: of top_p of their mass; top_p >= 1: all), and the pick by index.
+    __device__ void finish_list(const SampleArgs& a, int r, int rank, int total, int k, float top_p, int64_t limit) {
+        gather();
+        const int e = threadIdx.x >> 1, half = threadIdx.x & 1;
+        const bool real = e < total;
+        const Element me = real ? cuts->all[e] : Element{0, 0};
+        int64_t before = 0;
+        int place = 0;
+        for (int j = half; j < total; j += 2) {
+            const Element o = cuts->all[j];
+            if (o.c > me.c) {
+                before += o.w;
+                ++place;
+            }
+        }
+        before += __shfl_xor_sync(~0u, before, 1);
+        place += __shfl_xor_sync(~0u, place, 1);
+        const auto add = [](int64_t p, int64_t q) { return p + q; };
+        bool in = real && me.w > 0 && (k <= 0 || place < k);
+        if (top_p < 1.f) {
+            if (limit == 0) {
+                const int64_t mass = block_reduce<int64_t>(in && half == 0 ? me.w : 0, add, sh.part);
+                limit = limit_of(top_p, mass);
+            }
+            in = in && before < limit;
+        }
+        const int64_t mass = block_reduce<int64_t>(in && half == 0 ? me.w : 0, add, sh.part);
+        const int64_t pick = pick_of(a.u[r], mass);
+        if (half == 0 && real && !in) cuts->all[e].w = 0;
+        __syncthreads();
+        const uint32_t index = ~static_cast<uint32_t>(me.c);
+        int64_t run = 0;
+        for (int j = half; j < total; j += 2) {
+            const Element o = cuts->all[j];
+            if (~static_cast<uint32_t>(o.c) < index) run += o.w;
+        }
+        run += __shfl_xor_sync(~0u, run, 1);
+        if (rank == 0 && half == 0 && in && pick >= run && pick < run + me.w) {
+            a.token[r] = static_cast<int>(index);
+            if (a.logprob) a.logprob[r] = logf(static_cast<float>(me.w) / static_cast<float>(mass));
+        }
+        sync();  // no CTA leaves while another may read its lists
+    }
+    __device__ static int64_t limit_of(float top_p, int64_t mass) {
+        const int64_t limit = static_cast<int64_t>(ceil(static_cast<double>(top_p) * static_cast<double>(mass)));
+        return limit < 1 ? 1 : limit;
+    }
+    __device__ static int64_t pick_of(float u, int64_t mass) {
+        const int64_t pick = static_cast<int64_t>(static_cast<double>(u) * static_cast<double>(mass));
+        return pick < 0 ? 0 : pick > mass - 1 ? mass - 1 : pick;
     }
 
     // Lists the candidates that `in` takes; the cluster's number of them (the lists hold them all if it is <= kList).
@@ -235,28 +331,97 @@ struct Row {
         __syncthreads();
         each([&](float v, int i) {
             int64_t w;
-            if (in(v, i, &w)) {
+            // past the list's end only the fact counts, not how many
+            if (in(v, i, &w) && *const_cast<volatile int*>(&sh.board.listed) <= kList) {
                 const int at = atomicAdd(&sh.board.listed, 1);
                 if (at < kList) cuts->list[at] = Element{composite(v, first + i), w};
             }
         });
         sync();
         int total = 0;
+#pragma unroll
         for (int r = 0; r < CL; ++r) total += of(&sh.board, r)->listed;
         return total;
+    }
+
+    // Adds an element to the histograms.
+    template <bool MASS>
+    __device__ void count_in(int bin, int64_t w) {
+        atomicAdd(&cuts->hist[0][bin], 1u);
+        if (MASS) {
+            if (w & 0x3fff) atomicAdd(&cuts->hist[1][bin], static_cast<uint32_t>(w & 0x3fff));
+            if (w >> 14 & 0x3fff) atomicAdd(&cuts->hist[2][bin], static_cast<uint32_t>(w >> 14 & 0x3fff));
+            if (w >> 28) atomicAdd(&cuts->hist[3][bin], static_cast<uint32_t>(w >> 28));
+        }
+    }
+    // Sums the cluster's histograms and finds the bin in which the running measure, from `before` on, reaches `target`:
+    // sh.bin (-1: none), sh.before the measure before it, sh.cut_mass its number of elements.
+    template <bool MASS>
+    __device__ void find_bin(int64_t before, int64_t target) {
+        static_assert(kBins == 2 * kThreads, "two bins per thread");
+        if (threadIdx.x == 0) sh.bin = -1;
+        sync();
+        int64_t m0 = 0, m1 = 0;
+        uint32_t c0 = 0, c1 = 0;
+#pragma unroll
+        for (int r = 0; r < CL; ++r) {
+            const uint2* h = reinterpret_cast<const uint2*>(of(&cuts->hist[0][0], r)) + threadIdx.x;
+            const uint2 k = h[0];
+            c0 += k.x;
+            c1 += k.y;
+            if (MASS) {
+                const uint2 a = h[kBins / 2], b = h[kBins], c = h[kBins / 2 * 3];
+                m0 += a.x + (static_cast<int64_t>(b.x) << 14) + (static_cast<int64_t>(c.x) << 28);
+                m1 += a.y + (static_cast<int64_t>(b.y) << 14) + (static_cast<int64_t>(c.y) << 28);
+            }
+        }
+        if (!MASS) {
+            m0 = c0;
+            m1 = c1;
+        }
+        const int64_t end = before + block_inclusive(m0 + m1, sh.part), mid = end - m1, begin = mid - m0;
+        if (begin < target && end >= target) {
+            sh.bin = 2 * threadIdx.x + (mid >= target ? 0 : 1);
+            sh.before = mid >= target ? begin : mid;
+            sh.cut_mass = mid >= target ? c0 : c1;
+        }
+        __syncthreads();
+    }
+    __device__ void clear_bins() {
+        sync();  // the histograms have been read
+        for (int i = threadIdx.x; i < 4 * kBins; i += kThreads) (&cuts->hist[0][0])[i] = 0;
+        __syncthreads();
+    }
+
+    // Raises `low` to a logit above which the measure of the candidates is sure to reach `target`, because that of the
+    // threads' own largest ones alone does.  The likely tokens are few and mostly in shares of different threads, so few
+    // others are left above it, whatever the vocabulary's size.
+    template <bool MASS>
+    __device__ void raise_low(int64_t target, float own_top) {
+        if (!MASS && target > CL * kThreads / 2) return;
+        clear_bins();
+        if (!(own_top < low)) {
+            // of a cut's ties it counts as the last, whichever it is
+            const int64_t w = MASS ? weigh(own_top, -1 - first) : 1;
+            if (w > 0) count_in<MASS>(bin_of(own_top), w);
+        }
+        find_bin<MASS>(0, target);
+        // the bin's far edge, and a little more for the roundings
+        if (sh.bin >= 0 && sh.bin < kBins - 1) {
+            low = fmaxf(low, top - t * ((sh.bin + 1) * (kReach / kBins) * 1.0001f));
+            raised = true;
+        }
     }
 
     // Finds the element at which the measure of the candidates, in falling order, reaches `target` (>= 1, at most the
     // whole): the count (MASS false: every element within reach is a candidate) or the mass (those of at least `least`).
     template <bool MASS>
-    __device__ int64_t find_cut(int64_t target, int64_t least) {
+    __device__ void find_cut(int64_t target, int64_t least) {
         uint64_t lo = 0, hi = ~0ull;  // range of composites that holds the element
         int shift = -1;               // bins: of the distance (-1), else of the composite's distance from hi
         int64_t before = 0;
         for (;;) {
-            sync();  // the histograms and the board have been read
-            for (int i = threadIdx.x; i < 4 * kBins; i += kThreads) (&cuts->hist[0][0])[i] = 0;
-            __syncthreads();
+            clear_bins();
             const auto place = [&](float v, int i, int64_t* w, int* bin) {
                 const uint64_t c = composite(v, first + i);
                 if (c < lo || c > hi) return false;
@@ -272,54 +437,11 @@ struct Row {
             each([&](float v, int i) {
                 int64_t w;
                 int b;
-                if (!place(v, i, &w, &b)) return;
-                atomicAdd(&cuts->hist[0][b], 1u);
-                if (MASS) {
-                    if (w & 0x3fff) atomicAdd(&cuts->hist[1][b], static_cast<uint32_t>(w & 0x3fff));
-                    if (w >> 14 & 0x3fff) atomicAdd(&cuts->hist[2][b], static_cast<uint32_t>(w >> 14 & 0x3fff));
-                    if (w >> 28) atomicAdd(&cuts->hist[3][b], static_cast<uint32_t>(w >> 28));
-                }
+                if (place(v, i, &w, &b)) count_in<MASS>(b, w);
             });
-            sync();
-            // each thread sums consecutive bins over the cluster; the thread in whose bins the target lies says which
-            constexpr int PER = kBins / kThreads;
-            int64_t mine[PER], sum = 0;
-            int counts[PER];
-#pragma unroll
-            for (int b = 0; b < PER; ++b) {
-                mine[b] = 0;
-                counts[b] = 0;
-            }
-            for (int r = 0; r < CL; ++r) {
-                const uint32_t* h = of(&cuts->hist[0][0], r);
-#pragma unroll
-                for (int b = 0; b < PER; ++b) {
-                    const int at = threadIdx.x * PER + b;
-                    const uint32_t k = h[at];
-                    counts[b] += k;
-                    if (MASS) {
-                        if (k)
-                            mine[b] += static_cast<int64_t>(h[kBins + at]) + (static_cast<int64_t>(h[2 * kBins + at]) << 14) +
-                                       (static_cast<int64_t>(h[3 * kBins + at]) << 28);
-                    } else {
-                        mine[b] += k;
-                    }
-                }
-            }
-#pragma unroll
-            for (int b = 0; b < PER; ++b) sum += mine[b];
-            int64_t run = before + block_inclusive(sum, sh.part) - sum;
-#pragma unroll
-            for (int b = 0; b < PER; ++b) {
-                if (run < target && run + mine[b] >= target) {
-                    sh.bin = threadIdx.x * PER + b;
-                    sh.before = run;
-                    sh.cut_mass = counts[b];
-                }
-                run += mine[b];
-            }
-            __syncthreads();
+            find_bin<MASS>(before, target);
             const int bin = sh.bin;
+            if (bin < 0) return;  // not reached: the callers ask for less than there is
             before = sh.before;
             const int64_t in_bin = sh.cut_mass;
             const auto inside = [&](float v, int i, int64_t* w) {
@@ -328,7 +450,8 @@ struct Row {
             };
             if (in_bin <= kList) {
                 const int total = list(inside);
-                return rank_list<MASS>(before, target, total);
+                rank_list<MASS>(before, target, total);
+                return;
             }
             // too many for the list: divide the range of their composites
             uint64_t a = ~0ull, z = 0;
@@ -369,19 +492,12 @@ __global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) sample_kernel(SampleAr
     const int first = rank * slice, n = max(0, min(a.vocab - first, slice));
     const T* from = static_cast<const T*>(a.logits) + r * a.row_stride + first;
 
-    // -- read the slice once: 16 bytes at a time where the row allows it --
-    constexpr int V = 16 / sizeof(T);
-    uint64_t best = 0;
-    const int head = static_cast<int>(min(static_cast<int64_t>(n), static_cast<int64_t>(
-                                                                       (16 - (reinterpret_cast<uintptr_t>(from) & 15)) & 15) /
-                                                                       static_cast<int64_t>(sizeof(T))));
-    const int packs = (n - head) / V;
-    const auto take = [&](T v, int i) {
-        x[i] = v;
-        best = max(best, composite(as_float(v), first + i));
-    };
-    for (int i = threadIdx.x; i < head; i += kThreads) take(from[i], i);
-    constexpr int U = 4;
+    // -- read the slice once: 16 bytes at a time between its ragged ends, to the same offset from a 16-byte boundary --
+    constexpr int V = 16 / sizeof(T), U = 4;
+    const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(from) & 15);
+    x = reinterpret_cast<T*>(reinterpret_cast<char*>(x) + skew);
+    const int head = min(n, ((16 - skew) & 15) / static_cast<int>(sizeof(T))), packs = (n - head) / V;
+    float top = -INFINITY;  // fmaxf passes over NaN
     for (int p0 = threadIdx.x; p0 < packs; p0 += kThreads * U) {
         uint4 w[U];
 #pragma unroll
@@ -390,30 +506,49 @@ __global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) sample_kernel(SampleAr
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (p0 + u * kThreads >= packs) continue;
+            reinterpret_cast<uint4*>(x + head)[p0 + u * kThreads] = w[u];
             const T* v = reinterpret_cast<const T*>(&w[u]);
 #pragma unroll
-            for (int k = 0; k < V; ++k) take(v[k], head + (p0 + u * kThreads) * V + k);
+            for (int k = 0; k < V; ++k) top = fmaxf(top, as_float(v[k]));
         }
     }
-    for (int i = head + packs * V + threadIdx.x; i < n; i += kThreads) take(from[i], i);
-    best = block_reduce(best, [](uint64_t p, uint64_t q) { return max(p, q); }, sh.part64);
-
+    const int ends = n - packs * V;  // the head, then what the packs leave
+    for (int j = threadIdx.x; j < ends; j += kThreads) {
+        const int i = j < head ? j : j + packs * V;
+        x[i] = from[i];
+        top = fmaxf(top, as_float(x[i]));
+    }
+    const float own_top = top;  // of this thread's elements
+    const auto larger = [](float p, float q) { return fmaxf(p, q); };
+    top = block_reduce(top, larger, reinterpret_cast<float*>(sh.part));
     Row<T, CL, CUTS> row{x, sh, cuts, first, n};
-    if (threadIdx.x == 0) sh.board.best = best;
+    if (threadIdx.x == 0) sh.board.top = top;
     row.sync();
-    for (int c = 0; c < CL; ++c) best = max(best, row.of(&sh.board, c)->best);
-    row.top = value_of(static_cast<uint32_t>(best >> 32));
+#pragma unroll
+    for (int c = 0; c < CL; ++c) top = fmaxf(top, row.of(&sh.board, c)->top);
+    row.top = top;
     const float temperature = a.temperature ? a.temperature[r] : 1.f;
-    const bool none = row.top == -INFINITY, greedy = !(temperature > 0.f);
+    const bool none = top == -INFINITY, greedy = !(temperature > 0.f);
     if (none || greedy) {
+        int at = INT32_MAX;  // the first of the largest
+        for (int i = threadIdx.x; i < n && !none; i += kThreads)
+            if (as_float(x[i]) == top) {
+                at = first + i;
+                break;
+            }
+        at = block_reduce(at, [](int p, int q) { return min(p, q); }, reinterpret_cast<int*>(sh.part));
+        if (threadIdx.x == 0) sh.board.index = at;
+        row.sync();
         if (rank == 0 && threadIdx.x == 0) {
-            a.token[r] = none ? -1 : static_cast<int>(~static_cast<uint32_t>(best));
+            for (int c = 0; c < CL; ++c) at = min(at, row.of(&sh.board, c)->index);
+            a.token[r] = none ? -1 : at;
             if (a.logprob) a.logprob[r] = none ? -INFINITY : 0.f;
         }
         row.sync();  // no CTA leaves while another may read its board
         return;
     }
     row.t = temperature;
+    row.inv = temperature > 9.094947e-13f && temperature < 1.0995e12f ? __frcp_rn(temperature) : 0.f;
     row.min_p = a.min_p ? fminf(a.min_p[r], 1.f) : 0.f;
     // NaN, where both are infinite, takes everything
     row.low = row.top - (kReach + 0.5f) * temperature;
@@ -422,14 +557,25 @@ __global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) sample_kernel(SampleAr
     if constexpr (CUTS) {
         const int k = a.top_k ? a.top_k[r] : 0;
         const float top_p = a.top_p ? a.top_p[r] : 1.f;
+        const auto weighed = [&](float v, int i, int64_t* w) {
+            *w = row.weigh(v, i);
+            return true;
+        };
         if (k > 0) {
+            row.template raise_low<false>(k, own_top);
+            const int total = row.list(weighed);
+            if (total <= kList) {
+                row.finish_list(a, r, rank, total, k, top_p, 0);
+                return;
+            }
             // fewer within reach than k: no cut
             int near = 0;
             row.each([&](float, int) { ++near; });
-            near = static_cast<int>(block_reduce<int64_t>(near, [](int64_t p, int64_t q) { return p + q; }, sh.part));
+            near = block_reduce(near, [](int p, int q) { return p + q; }, reinterpret_cast<int*>(sh.part));
             if (threadIdx.x == 0) sh.board.count[2] = near;
             row.sync();
             near = 0;
+#pragma unroll
             for (int c = 0; c < CL; ++c) near += row.of(&sh.board, c)->count[2];
             if (k < near) {
                 row.template find_cut<false>(k, 0);
@@ -438,9 +584,17 @@ __global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) sample_kernel(SampleAr
         }
         row.weigh_regions(0, &mass, &count);
         if (top_p < 1.f) {
-            int64_t limit = static_cast<int64_t>(ceil(static_cast<double>(top_p) * static_cast<double>(mass)));
-            if (limit < 1) limit = 1;
+            const int64_t limit = row.limit_of(top_p, mass);
             if (limit < mass) {
+                const float reach = row.low;
+                row.template raise_low<true>(limit, own_top);
+                if (row.low > reach || a.vocab <= kList) {
+                    const int total = row.list(weighed);
+                    if (total <= kList) {
+                        row.finish_list(a, r, rank, total, 0, top_p, limit);
+                        return;
+                    }
+                }
                 // weights below (1 - p) mass / (2 count) are together less than what stays out
                 const double least = 0.5 * (1.0 - static_cast<double>(top_p)) * static_cast<double>(mass) / count;
                 row.template find_cut<true>(limit, static_cast<int64_t>(fmax(least, 0.0)));
@@ -453,9 +607,7 @@ __global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) sample_kernel(SampleAr
     }
 
     // -- the pick: the CTA, then the warp's region, then the element --
-    int64_t pick = static_cast<int64_t>(static_cast<double>(a.u[r]) * static_cast<double>(mass));
-    if (pick > mass - 1) pick = mass - 1;
-    if (pick < 0) pick = 0;
+    const int64_t pick = row.pick_of(a.u[r], mass);
     // this CTA's masses, as every CTA of the cluster knows its own
     int64_t mine = 0;
     for (int w = 0; w < kWarps; ++w) mine += sh.region[w];
@@ -493,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) sample_kernel(SampleAr
 
 template <typename T, int CL, bool CUTS>
 cudaError_t launch(const SampleArgs& a, int slice, cudaStream_t s) {
-    const int smem = slice * static_cast<int>(sizeof(T)) + (CUTS ? static_cast<int>(sizeof(SharedCut)) : 0);
+    const int smem = slice * static_cast<int>(sizeof(T)) + 16 + (CUTS ? static_cast<int>(sizeof(SharedCut)) : 0);
     static SmemOptIn opt_in;
     cudaError_t e = opt_in.once(reinterpret_cast<const void*>(sample_kernel<T, CL, CUTS>), kSampleMaxSmem);
     if (e != cudaSuccess) return e;
@@ -515,7 +667,7 @@ template <typename T, bool CUTS>
 cudaError_t launch_cluster(const SampleArgs& a, int sms, cudaStream_t s) {
     const int extra = CUTS ? static_cast<int>(sizeof(SharedCut)) : 0;
     const auto slice_of = [&](int cl) { return ((a.vocab + cl - 1) / cl + 7) & ~7; };
-    const auto bytes_of = [&](int cl) { return slice_of(cl) * static_cast<int64_t>(sizeof(T)) + extra; };
+    const auto bytes_of = [&](int cl) { return slice_of(cl) * static_cast<int64_t>(sizeof(T)) + 16 + extra; };
     const auto per_sm = [&](int cl) { return std::min<int64_t>(CUTS ? 2 : 3, (227 << 10) / (bytes_of(cl) + 2048)); };
     // Few rows: the most CTAs per row that the GPU holds at once.  More rows than that: the fewest that still let one
     // row be read while others on the SM are worked on.
