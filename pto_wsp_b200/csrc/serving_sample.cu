@@ -78,13 +78,12 @@ struct Shared {
     uint64_t part64[kWarps];
     int64_t region[kWarps];
     uint64_t cut;
-    int64_t cut_mass;
     int bin;
     int64_t before;
 };
 // only where a cut may be looked for
 struct SharedCut {
-    uint32_t hist[4][kBins];  // counts, and the masses' low 14, middle 14 and high bits: no sum passes 32 bits
+    uint32_t hist[3][kBins];  // counts, or the masses' low 14, middle 14 and high bits: no sum passes 32 bits
     Element list[kList];      // this CTA's share
     Element all[kList];       // the cluster's
 };
@@ -148,18 +147,20 @@ struct Row {
         return fmaf(fmaf(-q, t, a), inv, q);
     }
     __device__ float any_distance(float v) const { return inv != 0.f ? distance(v) : __fdiv_rn(v - top, t); }
-    // the candidate's weight, 0: none.  `v` is at or above `low`.
-    __device__ int64_t weigh(float v, int i) const {
+    // the candidate's weight, 0: none.  `v` is at or above `low`, `d` its distance.
+    __device__ int64_t weigh(float v, int i) const { return weigh(v, i, any_distance(v)); }
+    __device__ int64_t weigh(float v, int i, float d) const {
         float w = 1.f;
         if (v != top) {
-            w = expf(any_distance(v));
+            w = expf(d);
             if (!(w >= min_p) || !(v > -INFINITY)) return 0;
         }
         if (CUTS && composite(v, first + i) < cut) return 0;
         return whole_of(w);
     }
-    __device__ int bin_of(float v) const {
-        const float b = -any_distance(v) * kBinsPerUnit;
+    __device__ int bin_of(float v) const { return bin_at(any_distance(v)); }
+    __device__ static int bin_at(float d) {
+        const float b = -d * kBinsPerUnit;
         return b < kBins ? static_cast<int>(b) : kBins - 1;  // NaN (an infinite row's rest) is in the last bin
     }
 
@@ -323,12 +324,22 @@ struct Row {
         return pick < 0 ? 0 : pick > mass - 1 ? mass - 1 : pick;
     }
 
+    __device__ bool near_few() const {
+        int k = 0;
+        each([&](float, int) { ++k; });
+        return block_reduce(k, [](int p, int q) { return p + q; }, reinterpret_cast<int*>(sh.part)) <= kList;
+    }
+
     // Lists the candidates that `in` takes; the cluster's number of them (the lists hold them all if it is <= kList).
+    // `sure`: `in` takes whatever is at or above `low`, so that counting these tells a list that is too short.
     template <typename F>
-    __device__ int list(F in) {
+    __device__ int list(bool sure, F in) {
         sync();  // the last list has been read
         if (threadIdx.x == 0) sh.board.listed = 0;
         __syncthreads();
+        if (sure && !near_few()) {
+            if (threadIdx.x == 0) sh.board.listed = kList + 1;
+        } else
         each([&](float v, int i) {
             int64_t w;
             // past the list's end only the fact counts, not how many
@@ -344,52 +355,47 @@ struct Row {
         return total;
     }
 
-    // Adds an element to the histograms.
+    // Adds an element to the histogram: to its count, or to the three parts of its mass.
     template <bool MASS>
     __device__ void count_in(int bin, int64_t w) {
-        atomicAdd(&cuts->hist[0][bin], 1u);
-        if (MASS) {
-            if (w & 0x3fff) atomicAdd(&cuts->hist[1][bin], static_cast<uint32_t>(w & 0x3fff));
-            if (w >> 14 & 0x3fff) atomicAdd(&cuts->hist[2][bin], static_cast<uint32_t>(w >> 14 & 0x3fff));
-            if (w >> 28) atomicAdd(&cuts->hist[3][bin], static_cast<uint32_t>(w >> 28));
+        if (!MASS) {
+            atomicAdd(&cuts->hist[0][bin], 1u);
+            return;
         }
+        if (w & 0x3fff) atomicAdd(&cuts->hist[0][bin], static_cast<uint32_t>(w & 0x3fff));
+        if (w >> 14 & 0x3fff) atomicAdd(&cuts->hist[1][bin], static_cast<uint32_t>(w >> 14 & 0x3fff));
+        if (w >> 28) atomicAdd(&cuts->hist[2][bin], static_cast<uint32_t>(w >> 28));
     }
     // Sums the cluster's histograms and finds the bin in which the running measure, from `before` on, reaches `target`:
-    // sh.bin (-1: none), sh.before the measure before it, sh.cut_mass its number of elements.
+    // sh.bin (-1: none) and sh.before, the measure before it.
     template <bool MASS>
     __device__ void find_bin(int64_t before, int64_t target) {
         static_assert(kBins == 2 * kThreads, "two bins per thread");
         if (threadIdx.x == 0) sh.bin = -1;
         sync();
         int64_t m0 = 0, m1 = 0;
-        uint32_t c0 = 0, c1 = 0;
 #pragma unroll
         for (int r = 0; r < CL; ++r) {
             const uint2* h = reinterpret_cast<const uint2*>(of(&cuts->hist[0][0], r)) + threadIdx.x;
-            const uint2 k = h[0];
-            c0 += k.x;
-            c1 += k.y;
+            const uint2 a = h[0];
+            m0 += a.x;
+            m1 += a.y;
             if (MASS) {
-                const uint2 a = h[kBins / 2], b = h[kBins], c = h[kBins / 2 * 3];
-                m0 += a.x + (static_cast<int64_t>(b.x) << 14) + (static_cast<int64_t>(c.x) << 28);
-                m1 += a.y + (static_cast<int64_t>(b.y) << 14) + (static_cast<int64_t>(c.y) << 28);
+                const uint2 b = h[kBins / 2], c = h[kBins];
+                m0 += (static_cast<int64_t>(b.x) << 14) + (static_cast<int64_t>(c.x) << 28);
+                m1 += (static_cast<int64_t>(b.y) << 14) + (static_cast<int64_t>(c.y) << 28);
             }
-        }
-        if (!MASS) {
-            m0 = c0;
-            m1 = c1;
         }
         const int64_t end = before + block_inclusive(m0 + m1, sh.part), mid = end - m1, begin = mid - m0;
         if (begin < target && end >= target) {
             sh.bin = 2 * threadIdx.x + (mid >= target ? 0 : 1);
             sh.before = mid >= target ? begin : mid;
-            sh.cut_mass = mid >= target ? c0 : c1;
         }
         __syncthreads();
     }
     __device__ void clear_bins() {
         sync();  // the histograms have been read
-        for (int i = threadIdx.x; i < 4 * kBins; i += kThreads) (&cuts->hist[0][0])[i] = 0;
+        for (int i = threadIdx.x; i < 3 * kBins; i += kThreads) (&cuts->hist[0][0])[i] = 0;
         __syncthreads();
     }
 
@@ -422,34 +428,32 @@ struct Row {
         int64_t before = 0;
         for (;;) {
             clear_bins();
-            const auto place = [&](float v, int i, int64_t* w, int* bin) {
+            // the bin of an element in range, -1 if it is not; its distance in *d
+            const auto place = [&](float v, int i, float* d) -> int {
                 const uint64_t c = composite(v, first + i);
-                if (c < lo || c > hi) return false;
-                if (MASS) {
-                    *w = weigh(v, i);
-                    if (*w < least || *w == 0) return false;
-                } else {
-                    *w = 0;
-                }
-                *bin = shift < 0 ? bin_of(v) : static_cast<int>((hi - c) >> shift);
-                return true;
+                if (c < lo || c > hi) return -1;
+                *d = any_distance(v);
+                return shift < 0 ? bin_at(*d) : static_cast<int>((hi - c) >> shift);
             };
             each([&](float v, int i) {
-                int64_t w;
-                int b;
-                if (place(v, i, &w, &b)) count_in<MASS>(b, w);
+                float d;
+                const int b = place(v, i, &d);
+                if (b < 0) return;
+                const int64_t w = MASS ? weigh(v, i, d) : 1;
+                if (!MASS || (w >= least && w > 0)) count_in<MASS>(b, w);
             });
             find_bin<MASS>(before, target);
             const int bin = sh.bin;
             if (bin < 0) return;  // not reached: the callers ask for less than there is
             before = sh.before;
-            const int64_t in_bin = sh.cut_mass;
             const auto inside = [&](float v, int i, int64_t* w) {
-                int b;
-                return place(v, i, w, &b) && b == bin;
+                float d;
+                if (place(v, i, &d) != bin) return false;
+                *w = MASS ? weigh(v, i, d) : 0;
+                return !MASS || (*w >= least && *w > 0);
             };
-            if (in_bin <= kList) {
-                const int total = list(inside);
+            const int total = list(false, inside);
+            if (total <= kList) {
                 rank_list<MASS>(before, target, total);
                 return;
             }
@@ -563,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) sample_kernel(SampleAr
         };
         if (k > 0) {
             row.template raise_low<false>(k, own_top);
-            const int total = row.list(weighed);
+            const int total = row.list(true, weighed);
             if (total <= kList) {
                 row.finish_list(a, r, rank, total, k, top_p, 0);
                 return;
@@ -589,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) sample_kernel(SampleAr
                 const float reach = row.low;
                 row.template raise_low<true>(limit, own_top);
                 if (row.low > reach || a.vocab <= kList) {
-                    const int total = row.list(weighed);
+                    const int total = row.list(true, weighed);
                     if (total <= kList) {
                         row.finish_list(a, r, rank, total, 0, top_p, limit);
                         return;
@@ -669,13 +673,14 @@ cudaError_t launch_cluster(const SampleArgs& a, int sms, cudaStream_t s) {
     const auto slice_of = [&](int cl) { return ((a.vocab + cl - 1) / cl + 7) & ~7; };
     const auto bytes_of = [&](int cl) { return slice_of(cl) * static_cast<int64_t>(sizeof(T)) + 16 + extra; };
     const auto per_sm = [&](int cl) { return std::min<int64_t>(CUTS ? 2 : 3, (227 << 10) / (bytes_of(cl) + 2048)); };
-    // Few rows: the most CTAs per row that the GPU holds at once.  More rows than that: the fewest that still let one
-    // row be read while others on the SM are worked on.
-    int cl = 0;
-    for (int c = kMaxCluster; c >= 1 && !cl; c /= 2)
-        if ((c == 1 || slice_of(c) >= 512) && static_cast<int64_t>(a.rows) * c <= per_sm(c) * sms) cl = c;
-    for (int c = 1; c <= kMaxCluster && !cl; c *= 2)
-        if (per_sm(c) >= (CUTS ? 2 : 3) || c == kMaxCluster) cl = c;
+    // Slices of 8000 elements or more: below that the cluster's barriers and remote reads cost more than the passes save
+    // (one row of 8000 with top-p: 7.5 us in one CTA, 10.9 in four, 16.9 in eight; of 50000: 112, 44, 47).  Few rows are
+    // spread over the SMs, one CTA each; many rows share them, so that one is read while another is worked on.
+    int cl = 1;
+    while (cl < kMaxCluster && (slice_of(cl) > 32768 || bytes_of(cl) > kSampleMaxSmem ||
+                                (static_cast<int64_t>(a.rows) * cl * 2 <= sms && slice_of(cl * 2) >= 8000) ||
+                                (static_cast<int64_t>(a.rows) * cl > sms && per_sm(cl) < 2 && slice_of(cl * 2) >= 8000)))
+        cl *= 2;
     if (bytes_of(cl) > kSampleMaxSmem) return cudaErrorInvalidValue;
     switch (cl) {
         case 1: return launch<T, 1, CUTS>(a, slice_of(1), s);
