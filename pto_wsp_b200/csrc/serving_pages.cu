@@ -160,10 +160,13 @@ __global__ void __launch_bounds__(kRsvThreads) reserve_kernel(ReserveArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Append.  One warp owns one run -- the new tokens of one page -- of one head of K or of V: it takes the largest |x|,
-// settles the page's scale and writes the codes, so no two warps share a scale and no atomic is needed.  A CTA looks
-// at `chunk` consecutive tokens; a token whose predecessor is in another page begins a run, which the CTA that holds
-// its first token writes to its end (at most a page).
+// Append.  A run -- the new tokens of one page -- of one head of K or of V belongs to one team of 1, 2 or 4 warps: it takes
+// the largest |x|, settles the page's scale and writes the codes, so no two teams share a scale and no atomic is
+// needed.  A CTA looks at `chunk` consecutive tokens of one head; a token whose predecessor is in another page begins a
+// run, which the CTA that holds its first token writes to its end (at most a page).  Many short runs (decoding): a warp
+// each; few long ones (prefill): the warps share each, so that its rows are all under way at once and are read once.
+//
+// Bound by HBM: 2 or 4 bytes in and 1 out per element.
 // ---------------------------------------------------------------------------
 
 constexpr int kAppWarps = 8;
@@ -198,30 +201,70 @@ __device__ __forceinline__ void unpack16<__nv_bfloat16>(const uint4& w, float (&
     }
 }
 
-// Codes of 4 values x / scale, x not NaN.  `inv` is the reciprocal of a power of two (the product is then the exact
-// quotient), or 0: divide.
-template <int FMT>
-__device__ __forceinline__ uint32_t encode4(float x0, float x1, float x2, float x3, float scale, float inv) {
-    float v[4] = {x0, x1, x2, x3};
+// The largest |x| of 16-byte loads as a bit pattern, which orders like the magnitude, infinity and NaN above all.
+template <typename T>
+struct Largest {  // 16-bit types: two at a time
+    uint32_t bits = 0;
+    __device__ __forceinline__ void add(const uint4& w) {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = inv != 0.f ? v[i] * inv : __fdiv_rn(v[i], scale);
+        for (int i = 0; i < 4; ++i) {
+            if (sizeof(T) == 4) bits = max(bits, u[i] & 0x7fffffffu);
+            else bits = __vmaxu2(bits, u[i] & 0x7fff7fffu);
+        }
+    }
+    // over the warp, as f32; *finite: no infinity and no NaN among them
+    __device__ __forceinline__ float of_warp(bool* finite) const;
+};
+template <>
+__device__ __forceinline__ float Largest<float>::of_warp(bool* finite) const {
+    const uint32_t m = __reduce_max_sync(~0u, bits);
+    *finite = m < 0x7f800000u;
+    return __uint_as_float(m);
+}
+template <>
+__device__ __forceinline__ float Largest<__half>::of_warp(bool* finite) const {
+    const uint32_t m = __reduce_max_sync(~0u, max(bits & 0xffffu, bits >> 16));
+    *finite = m < 0x7c00u;
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(m)));
+}
+template <>
+__device__ __forceinline__ float Largest<__nv_bfloat16>::of_warp(bool* finite) const {
+    const uint32_t m = __reduce_max_sync(~0u, max(bits & 0xffffu, bits >> 16));
+    *finite = m < 0x7f80u;
+    return __uint_as_float(m << 16);
+}
+
+// Codes of 4 values x / scale, x not NaN; inv = RN(1 / scale), `exact` where that is exact (a power of two).  int8: the
+// product is within 2^-16 of the quotient, so it rounds to the same integer unless it is that near to a half; only
+// there the quotient itself is taken.  Adding 1.5 * 2^23 rounds to the nearest even integer and leaves it in the low bits
+// (the conversion instructions have a quarter of an addition's rate).
+template <int FMT>
+__device__ __forceinline__ uint32_t encode4(float x0, float x1, float x2, float x3, float scale, float inv, bool exact) {
+    float v[4] = {x0, x1, x2, x3};
     if (FMT == PTOWSP_KV8_E4M3) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = exact ? v[i] * inv : __fdiv_rn(v[i], scale);
         const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3);
         const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3);
         return lo | (hi << 16);
     }
-    uint32_t r = 0;
+    constexpr float kMagic = 12582912.f;
+    uint32_t t[4];
+    float far = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int c = static_cast<int>(rintf(fminf(fmaxf(v[i], -127.f), 127.f)));
-        r |= (static_cast<uint32_t>(c) & 0xffu) << (8 * i);
+        const float q = fminf(fmaxf(v[i] * inv, -127.f), 127.f);
+        const float r = q + kMagic;
+        t[i] = __float_as_uint(r);
+        far = fmaxf(far, fabsf(q - (r - kMagic)));
     }
-    return r;
-}
-
-// 1 / s for a power of two, else 0.
-__device__ __forceinline__ float exact_inverse(float s) {
-    return (__float_as_uint(s) & 0x007fffffu) == 0 ? __fdiv_rn(1.f, s) : 0.f;
+    if (far > 0.49997f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            t[i] = __float_as_uint(fminf(fmaxf(__fdiv_rn(v[i], scale), -127.f), 127.f) + kMagic);
+    }
+    return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
 }
 
 template <int FMT>
@@ -234,56 +277,76 @@ __device__ __forceinline__ float scale_for(float amax) {
     return ldexpf(1.f, min(max(e, -60), 60));
 }
 
+// Warp `sub` of a team of `team` on one run.  `part`: a float per warp of the block.  Every warp of the block comes here
+// (with run 0 where it has none) when the team is more than one warp, for the barriers.
 template <typename T, int FMT, int D>
-__device__ void append_run(const Kv8Side& c, int64_t page, int head, int heads, int page_size, const char* x,
-                           int64_t token_stride, const int64_t* slots, int64_t i0, int run, int lane) {
+__device__ __forceinline__ void append_run(const Kv8Side& c, int64_t page, int head, int heads, int page_size, const char* x,
+                                           int64_t token_stride, const int64_t* slots, int64_t i0, int run, int sub,
+                                           int team, float* part) {
     constexpr int V = 16 / sizeof(T);       // elements per 16-byte load
     constexpr int LPT = D / V;              // lanes per token
     constexpr int TPW = 32 / LPT;           // tokens per warp load
     constexpr int U = 8;                    // loads in flight
-    const int sub = lane / LPT, el = (lane % LPT) * V;
-    const T* src = reinterpret_cast<const T*>(x) + el;
-    // offsets that the run writes, and its largest finite |x|
-    uint32_t mask[4] = {0, 0, 0, 0};
-    for (int j = lane; j < run; j += 32) {
-        const int off = static_cast<int>(slots[i0 + j] & (page_size - 1));
-        mask[off >> 5] |= 1u << (off & 31);
-    }
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mask[w] = __reduce_or_sync(~0u, mask[w]);
-    float amax = 0.f;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int el = (lane % LPT) * V;
+    const T* src = reinterpret_cast<const T*>(x) + el + i0 * token_stride;
+    // token of load s of this lane
+    const auto token = [&](int s) { return (s * team + sub) * TPW + lane / LPT; };
+    const int steps = (run + TPW * team - 1) / (TPW * team);
     uint4 raw[U];
-    const int steps = (run + TPW - 1) / TPW;
+    Largest<T> largest;
     for (int s0 = 0; s0 < steps; s0 += U) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = (s0 + u) * TPW + sub;
+            const int j = token(s0 + u);
             raw[u] = make_uint4(0, 0, 0, 0);
-            if (j < run) raw[u] = *reinterpret_cast<const uint4*>(src + (i0 + j) * token_stride);
+            if (j < run) raw[u] = *reinterpret_cast<const uint4*>(src + j * token_stride);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float f[V];
-            unpack16<T>(raw[u], f);
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float m = fabsf(f[k]);
-                amax = m < INFINITY ? fmaxf(amax, m) : amax;
-            }
-        }
+        for (int u = 0; u < U; ++u) largest.add(raw[u]);
     }
-    amax = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(amax)));  // ordered: not negative
+    bool finite;
+    float amax = largest.of_warp(&finite);
+    if (!finite) {  // look again, at the finite ones
+        amax = 0.f;
+        for (int s = 0; s < steps; ++s) {
+            const int j = token(s);
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (j < run) w = *reinterpret_cast<const uint4*>(src + j * token_stride);
+            float f[V];
+            unpack16<T>(w, f);
+#pragma unroll
+            for (int k = 0; k < V; ++k) amax = fabsf(f[k]) < INFINITY ? fmaxf(amax, fabsf(f[k])) : amax;
+        }
+        amax = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(amax)));  // ordered: not negative
+    }
     float* scale_at = c.scale + page * heads + head;
-    const bool fresh = mask[0] & 1u;
-    const float old = *scale_at;
+    const float old = run ? *scale_at : 1.f;
+    if (team > 1) {
+        if (lane == 0) part[warp] = amax;
+        __syncthreads();
+        for (int w = warp - sub; w < warp - sub + team; ++w) amax = fmaxf(amax, part[w]);
+    }
+    if (!run) return;
+    // a run's slots ascend, so its first one tells whether it holds the page's token 0
+    const bool fresh = (slots[i0] & (page_size - 1)) == 0;
     const float need = scale_for<FMT>(amax);
     const float scale = fresh ? need : fmaxf(old, need);
-    const float inv = exact_inverse(scale);
+    const float inv = __frcp_rn(scale);
+    const bool exact = (__float_as_uint(scale) & 0x007fffffu) == 0;
     uint8_t* base = c.codes + page * c.page_stride + head * c.head_stride;
     if (!fresh && scale > old) {  // round the page's other codes to the new scale
-        constexpr int LPR = D / 16;  // lanes per row of codes
-        for (int off = lane / LPR; off < page_size; off += 32 / LPR) {
-            if (mask[off >> 5] >> (off & 31) & 1u) continue;
+        uint32_t mask[4] = {0, 0, 0, 0};  // offsets that the run writes
+        for (int j = lane; j < run; j += 32) {
+            const int off = static_cast<int>(slots[i0 + j] & (page_size - 1));
+            mask[off >> 5] |= 1u << (off & 31);
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mask[w] = __reduce_or_sync(~0u, mask[w]);
+        constexpr int LPR = D / 16, RPW = 32 / LPR;  // lanes per row of codes, rows per warp
+        for (int off = sub * RPW + lane / LPR; off < page_size; off += team * RPW) {
+            const uint32_t word = off < 32 ? mask[0] : off < 64 ? mask[1] : off < 96 ? mask[2] : mask[3];
+            if (word >> (off & 31) & 1u) continue;
             uint4* p = reinterpret_cast<uint4*>(base + off * c.token_stride + (lane % LPR) * 16);
             uint4 w = *p;
             uint32_t* u = reinterpret_cast<uint32_t*>(&w);
@@ -291,34 +354,36 @@ __device__ void append_run(const Kv8Side& c, int64_t page, int head, int heads, 
             for (int k = 0; k < 4; ++k) {
                 float f[4];
                 decode4<FMT>(u[k], f);
-                u[k] = encode4<FMT>(f[0] * old, f[1] * old, f[2] * old, f[3] * old, scale, inv);
+                u[k] = encode4<FMT>(f[0] * old, f[1] * old, f[2] * old, f[3] * old, scale, inv, exact);
             }
             *p = w;
         }
     }
-    __syncwarp();
-    if (lane == 0) *scale_at = scale;
+    __syncwarp();  // the old scale has been read, by the team's other warps before the barrier above
+    if (sub == 0 && lane == 0) *scale_at = scale;
     for (int s0 = 0; s0 < steps; s0 += U) {
-        if (steps > U) {  // a long run is read again (it is in the cache); a short one is still in registers
+        if (steps > U) {  // a share of more than U loads is read again (it is in the cache); else it is in registers
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int j = (s0 + u) * TPW + sub;
+                const int j = token(s0 + u);
                 raw[u] = make_uint4(0, 0, 0, 0);
-                if (j < run) raw[u] = *reinterpret_cast<const uint4*>(src + (i0 + j) * token_stride);
+                if (j < run) raw[u] = *reinterpret_cast<const uint4*>(src + j * token_stride);
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = (s0 + u) * TPW + sub;
+            const int j = token(s0 + u);
             if (j >= run) continue;
             float f[V];
             unpack16<T>(raw[u], f);
+            if (!finite) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) f[k] = f[k] == f[k] ? f[k] : 0.f;
+                for (int k = 0; k < V; ++k) f[k] = f[k] == f[k] ? f[k] : 0.f;
+            }
             uint32_t out[V / 4];
 #pragma unroll
             for (int k = 0; k < V / 4; ++k)
-                out[k] = encode4<FMT>(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3], scale, inv);
+                out[k] = encode4<FMT>(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3], scale, inv, exact);
             const int off = static_cast<int>(slots[i0 + j] & (page_size - 1));
             uint8_t* to = base + off * c.token_stride + el;
             if constexpr (V == 8) *reinterpret_cast<uint2*>(to) = make_uint2(out[0], out[1]);
@@ -328,50 +393,70 @@ __device__ void append_run(const Kv8Side& c, int64_t page, int head, int heads, 
 }
 
 template <typename T, int FMT, int D>
-__global__ void __launch_bounds__(kAppWarps * 32) append_kernel(AppendArgs a, int chunk) {
-    __shared__ int first[kAppMaxChunk], length[kAppMaxChunk];
+__global__ void __launch_bounds__(kAppWarps * 32, 4) append_kernel(AppendArgs a, int chunk) {
+    __shared__ int first[kAppMaxChunk], length[kAppMaxChunk], page_of[kAppMaxChunk];
     __shared__ int runs;
+    __shared__ float part[kAppWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t c0 = static_cast<int64_t>(blockIdx.x) * chunk;
     const int heads = a.cache.kv_heads, shift = a.cache.page_shift, page_size = a.cache.page_size;
-    const int64_t limit = a.cache.pages << shift;
+    const int head = blockIdx.y;
     if (warp == 0) {
-        const int64_t i = c0 + lane;
-        bool begins = false;
-        int len = 0;
-        if (lane < chunk && i < a.tokens) {
-            const int64_t s = a.slots[i];
+        const int64_t limit = a.cache.pages << shift;
+        // whether token i goes on with the run of token i - 1, and its slot
+        const auto look = [&](int64_t i, bool* goes_on) -> int64_t {
+            const int64_t s = i < a.tokens ? a.slots[i] : -1;
+            const int64_t before = i > 0 && i <= a.tokens ? a.slots[i - 1] : -1;
             const bool ok = s >= 0 && s < limit;
-            if (!ok && s != -1 && a.status) atomicOr(a.status, PTOWSP_SERVING_PAGE);
-            const int64_t before = i ? a.slots[i - 1] : -1;
-            begins = ok && (before < 0 || (before >> shift) != (s >> shift) || before >= s);
-            if (begins) {
-                int64_t last = s;
-                for (len = 1; i + len < a.tokens; ++len) {
-                    const int64_t n = a.slots[i + len];
-                    if (n <= last || (n >> shift) != (s >> shift)) break;
-                    last = n;
-                }
-            }
-        }
-        const uint32_t all = __ballot_sync(~0u, begins);
-        if (begins) {
-            const int k = __popc(all & ((1u << lane) - 1u));
+            *goes_on = ok && before >= 0 && before < s && (before >> shift) == (s >> shift);
+            return ok ? s : s == -1 ? -1 : -2;
+        };
+        bool goes_on;
+        const int64_t s = look(c0 + lane, &goes_on);
+        const bool here = lane < chunk;
+        if (here && s == -2 && a.status) atomicOr(a.status, PTOWSP_SERVING_PAGE);
+        const uint32_t begins = __ballot_sync(~0u, here && s >= 0 && !goes_on);
+        const uint32_t breaks = __ballot_sync(~0u, here && !goes_on);
+        if (begins >> lane & 1u) {
+            const int k = __popc(begins & ((1u << lane) - 1u));
+            const uint32_t later = lane == 31 ? 0u : breaks >> (lane + 1) << (lane + 1);
             first[k] = lane;
-            length[k] = len;
+            page_of[k] = static_cast<int>(s >> shift);
+            length[k] = (later ? __ffs(later) - 1 : chunk) - lane;
         }
-        if (lane == 0) runs = __popc(all);
+        if (lane == 0) runs = __popc(begins);
+        // the run that holds the chunk's last token may go on behind it, to the end of its page at most
+        const bool open = begins && __clz(static_cast<int>(breaks)) == __clz(static_cast<int>(begins));
+        __syncwarp();
+        if (open) {
+            int more = 0;
+            for (int64_t i = c0 + chunk;; i += 32) {
+                look(i + lane, &goes_on);
+                const uint32_t stop = __ballot_sync(~0u, !goes_on);
+                if (stop) {
+                    more += __ffs(stop) - 1;
+                    break;
+                }
+                more += 32;
+            }
+            if (lane == 0) length[__popc(begins) - 1] += more;
+        }
     }
     __syncthreads();
-    const int head = blockIdx.y;
-    for (int it = warp; it < runs * 2; it += kAppWarps) {
-        const int which = it & 1, k = it >> 1;
+    const int items = runs * 2;
+    const int team = items > kAppWarps / 2 ? 1 : items > kAppWarps / 4 ? 2 : 4;
+    const int teams = kAppWarps / team;
+    for (int it0 = 0; it0 < items; it0 += teams) {
+        const int it = it0 + warp / team;
+        const bool live = it < items;
+        const int which = it & 1, k = live ? it >> 1 : 0;
         const int64_t i0 = c0 + first[k];
-        const int64_t page = a.slots[i0] >> shift;
         const char* x = static_cast<const char*>(which ? a.v : a.k) +
                         head * (which ? a.v_head_stride : a.k_head_stride) * static_cast<int64_t>(sizeof(T));
-        append_run<T, FMT, D>(which ? a.cache.v : a.cache.k, page, head, heads, page_size, x,
-                              which ? a.v_token_stride : a.k_token_stride, a.slots, i0, length[k], lane);
+        append_run<T, FMT, D>(which ? a.cache.v : a.cache.k, page_of[k], head, heads, page_size, x,
+                              which ? a.v_token_stride : a.k_token_stride, a.slots, i0, live ? length[k] : 0, warp % team,
+                              team, part);
+        if (team > 1) __syncthreads();  // `part` has been read
     }
 }
 
