@@ -210,7 +210,7 @@ struct Largest {  // 16-bit types: two at a time
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (sizeof(T) == 4) bits = max(bits, u[i] & 0x7fffffffu);
-            else bits = __vmaxu2(bits, u[i] & 0x7fff7fffu);
+            else asm("max.u16x2 %0, %0, %1;" : "+r"(bits) : "r"(u[i] & 0x7fff7fffu));
         }
     }
     // over the warp, as f32; *finite: no infinity and no NaN among them
@@ -239,14 +239,28 @@ __device__ __forceinline__ float Largest<__nv_bfloat16>::of_warp(bool* finite) c
 // product is within 2^-16 of the quotient, so it rounds to the same integer unless it is that near to a half; only
 // there the quotient itself is taken.  Adding 1.5 * 2^23 rounds to the nearest even integer and leaves it in the low bits
 // (the conversion instructions have a quarter of an addition's rate).
+__device__ __noinline__ uint32_t divide4(float x0, float x1, float x2, float x3, float scale) {
+    const float v[4] = {x0, x1, x2, x3};
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float q = fminf(fmaxf(__fdiv_rn(v[i], scale), -127.f), 127.f);
+        r |= (__float_as_uint(q + 12582912.f) & 0xffu) << (8 * i);
+    }
+    return r;
+}
+__device__ __noinline__ uint32_t divide4_e4m3(float x0, float x1, float x2, float x3, float scale) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x0, scale), __fdiv_rn(x1, scale)), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x2, scale), __fdiv_rn(x3, scale)), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+}
 template <int FMT>
 __device__ __forceinline__ uint32_t encode4(float x0, float x1, float x2, float x3, float scale, float inv, bool exact) {
-    float v[4] = {x0, x1, x2, x3};
+    const float v[4] = {x0, x1, x2, x3};
     if (FMT == PTOWSP_KV8_E4M3) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = exact ? v[i] * inv : __fdiv_rn(v[i], scale);
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3);
+        if (!exact) return divide4_e4m3(x0, x1, x2, x3, scale);
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x0 * inv, x1 * inv), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x2 * inv, x3 * inv), __NV_SATFINITE, __NV_E4M3);
         return lo | (hi << 16);
     }
     constexpr float kMagic = 12582912.f;
@@ -259,11 +273,7 @@ __device__ __forceinline__ uint32_t encode4(float x0, float x1, float x2, float 
         t[i] = __float_as_uint(r);
         far = fmaxf(far, fabsf(q - (r - kMagic)));
     }
-    if (far > 0.49997f) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            t[i] = __float_as_uint(fminf(fmaxf(__fdiv_rn(v[i], scale), -127.f), 127.f) + kMagic);
-    }
+    if (far > 0.49997f) return divide4(x0, x1, x2, x3, scale);
     return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
 }
 
@@ -289,7 +299,8 @@ __device__ __forceinline__ void append_run(const Kv8Side& c, int64_t page, int h
     constexpr int U = 8;                    // loads in flight
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int el = (lane % LPT) * V;
-    const T* src = reinterpret_cast<const T*>(x) + el + i0 * token_stride;
+    const T* src = reinterpret_cast<const T*>(x) + el + (i0 + sub * TPW + lane / LPT) * token_stride;
+    const int64_t step = static_cast<int64_t>(team) * TPW * token_stride;  // between this lane's loads
     // token of load s of this lane
     const auto token = [&](int s) { return (s * team + sub) * TPW + lane / LPT; };
     const int steps = (run + TPW * team - 1) / (TPW * team);
@@ -300,7 +311,7 @@ __device__ __forceinline__ void append_run(const Kv8Side& c, int64_t page, int h
         for (int u = 0; u < U; ++u) {
             const int j = token(s0 + u);
             raw[u] = make_uint4(0, 0, 0, 0);
-            if (j < run) raw[u] = *reinterpret_cast<const uint4*>(src + j * token_stride);
+            if (j < run) raw[u] = *reinterpret_cast<const uint4*>(src + (s0 + u) * step);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) largest.add(raw[u]);
@@ -312,7 +323,7 @@ __device__ __forceinline__ void append_run(const Kv8Side& c, int64_t page, int h
         for (int s = 0; s < steps; ++s) {
             const int j = token(s);
             uint4 w = make_uint4(0, 0, 0, 0);
-            if (j < run) w = *reinterpret_cast<const uint4*>(src + j * token_stride);
+            if (j < run) w = *reinterpret_cast<const uint4*>(src + s * step);
             float f[V];
             unpack16<T>(w, f);
 #pragma unroll
@@ -367,7 +378,7 @@ __device__ __forceinline__ void append_run(const Kv8Side& c, int64_t page, int h
             for (int u = 0; u < U; ++u) {
                 const int j = token(s0 + u);
                 raw[u] = make_uint4(0, 0, 0, 0);
-                if (j < run) raw[u] = *reinterpret_cast<const uint4*>(src + j * token_stride);
+                if (j < run) raw[u] = *reinterpret_cast<const uint4*>(src + (s0 + u) * step);
             }
         }
 #pragma unroll
@@ -393,14 +404,15 @@ __device__ __forceinline__ void append_run(const Kv8Side& c, int64_t page, int h
 }
 
 template <typename T, int FMT, int D>
-__global__ void __launch_bounds__(kAppWarps * 32, 4) append_kernel(AppendArgs a, int chunk) {
+__global__ void __launch_bounds__(kAppWarps * 32, 4) append_kernel(const __grid_constant__ AppendArgs a, int chunk) {
     __shared__ int first[kAppMaxChunk], length[kAppMaxChunk], page_of[kAppMaxChunk];
     __shared__ int runs;
     __shared__ float part[kAppWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t c0 = static_cast<int64_t>(blockIdx.x) * chunk;
     const int heads = a.cache.kv_heads, shift = a.cache.page_shift, page_size = a.cache.page_size;
-    const int head = blockIdx.y;
+    // the heads of a token stand side by side in memory: their CTAs run at the same time
+    const int head = static_cast<int>(blockIdx.x % static_cast<unsigned>(heads));
+    const int64_t c0 = static_cast<int64_t>(blockIdx.x / static_cast<unsigned>(heads)) * chunk;
     if (warp == 0) {
         const int64_t limit = a.cache.pages << shift;
         // whether token i goes on with the run of token i - 1, and its slot
@@ -493,9 +505,9 @@ cudaError_t launch_append(const AppendArgs& a, cudaStream_t s) {
     // few tokens: two per CTA and head; many: 32
     int chunk = 2;
     while (chunk < kAppMaxChunk && a.tokens * a.cache.kv_heads > 592 * static_cast<int64_t>(chunk)) chunk *= 2;
-    const int64_t blocks = (a.tokens + chunk - 1) / chunk;
+    const int64_t blocks = (a.tokens + chunk - 1) / chunk * a.cache.kv_heads;
     if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.cache.kv_heads));
+    const dim3 grid(static_cast<unsigned>(blocks));
     switch (a.dtype) {
         case PTOWSP_F32: return append_t<float>(a, grid, chunk, s);
         case PTOWSP_F16: return append_t<__half>(a, grid, chunk, s);
