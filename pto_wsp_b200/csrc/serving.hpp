@@ -89,6 +89,7 @@ struct AttendArgs {
     const int32_t* kv_len;
     const int32_t* q_start;  // nullptr: one token per request
     int requests, heads, group, max_q, window;
+    int few;  // requests with more q rows (tokens x group) are left to launch_prefill; 0: none are
     int64_t tokens;
     float scale;
     char* workspace;
@@ -99,6 +100,10 @@ cudaError_t launch_attend(const AttendArgs& a, int sms, cudaStream_t s);
 
 constexpr int kSampleMaxSmem = 224 << 10;  // of a CTA: its slice of the row, histograms and lists
 constexpr int kSampleMaxVocab = 393216;    // eight slices of 192 KB of f32
+// Requests of more than `threshold` q rows, on tcgen05 (serving_prefill.cu).
+size_t prefill_workspace_bytes(const AttendArgs& a, int sms);
+cudaError_t launch_prefill(const AttendArgs& a, int threshold, char* workspace, int sms, cudaStream_t s);
+
 struct SampleArgs {
     const void* logits;
     int64_t row_stride;

@@ -126,6 +126,7 @@ __device__ __forceinline__ Request request_at(const AttendArgs& a, int r, int* f
             q.lo = q.seen & ~(kTile - 1);
         }
     }
+    if (a.few && static_cast<int64_t>(q.nq) * a.group > a.few) q.nq = 0;
     q.tasks = static_cast<int64_t>((static_cast<int64_t>(q.nq) * a.group + ROWS - 1) / ROWS) * a.cache.kv_heads;
     const int64_t span = q.hi - q.lo;
     q.units = span > 0 ? (span + kUnit - 1) / kUnit : 1;  // a task without keys still writes its zeros
@@ -849,24 +850,50 @@ cudaError_t launch_rows(const AttendArgs& a, int sms, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, attend_kernel<FMT, D, NB>, a, k_map, v_map);
 }
 
+// Fragments of 8 q rows per tile.  With requests left to the other kernel most of the rest have one token.
+int fragments(const AttendArgs& a) {
+    const int64_t rows = a.few ? a.group : static_cast<int64_t>(a.max_q) * a.group;
+    return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+}
+
 template <int FMT, int D>
 cudaError_t launch_d(const AttendArgs& a, int sms, cudaStream_t s) {
-    const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
-    if (rows <= 8) return launch_rows<FMT, D, 1>(a, sms, s);
-    if (rows <= 16) return launch_rows<FMT, D, 2>(a, sms, s);
-    return launch_rows<FMT, D, 4>(a, sms, s);
+    switch (fragments(a)) {
+        case 1: return launch_rows<FMT, D, 1>(a, sms, s);
+        case 2: return launch_rows<FMT, D, 2>(a, sms, s);
+        default: return launch_rows<FMT, D, 4>(a, sms, s);
+    }
+}
+
+// Above so many q rows of a request the tcgen05 kernel is faster although it pads them to 128: a tile of 32 rows takes
+// the warp MMAs about 1.4 times as long as its codes take from HBM, and every further tile as long again.
+constexpr int kFew = 32;
+
+size_t few_bytes(const AttendArgs& a, int sms) {
+    const int nb = fragments(a);
+    return (kArrivals + static_cast<size_t>(sms) * ctas_per_sm(nb) * 2 * (8 * nb) * (a.cache.head_dim + 2) * sizeof(float) +
+            255) / 256 * 256;
+}
+
+AttendArgs split(const AttendArgs& a) {
+    AttendArgs b = a;
+    b.few = static_cast<int64_t>(a.max_q) * a.group > kFew ? kFew : 0;
+    return b;
 }
 
 }  // namespace
 
-size_t attend_workspace_bytes(const AttendArgs& a, int sms) {
-    const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
-    const int nb = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-    return kArrivals + static_cast<size_t>(sms) * ctas_per_sm(nb) * 2 * (8 * nb) * (a.cache.head_dim + 2) * sizeof(float);
+size_t attend_workspace_bytes(const AttendArgs& args, int sms) {
+    const AttendArgs a = split(args);
+    return few_bytes(a, sms) + (a.few ? prefill_workspace_bytes(a, sms) : 0);
 }
 
-cudaError_t launch_attend(const AttendArgs& a, int sms, cudaStream_t s) {
-    if (a.requests == 0 || a.tokens == 0) return cudaSuccess;
+cudaError_t launch_attend(const AttendArgs& args, int sms, cudaStream_t s) {
+    if (args.requests == 0 || args.tokens == 0) return cudaSuccess;
+    const AttendArgs a = split(args);
+    cudaError_t e = cudaSuccess;
+    if (a.few) e = launch_prefill(a, kFew, a.workspace + few_bytes(a, sms), sms, s);
+    if (e != cudaSuccess) return e;
     if (a.cache.format == PTOWSP_KV8_E4M3)
         return a.cache.head_dim == 64 ? launch_d<PTOWSP_KV8_E4M3, 64>(a, sms, s) : launch_d<PTOWSP_KV8_E4M3, 128>(a, sms, s);
     return a.cache.head_dim == 64 ? launch_d<PTOWSP_KV8_INT8, 64>(a, sms, s) : launch_d<PTOWSP_KV8_INT8, 128>(a, sms, s);

@@ -1,0 +1,830 @@
+// Attention over a paged KV cache held in 8 bits, for many query rows per request (prefill chunks), on tcgen05.
+//
+// The mathematics is that of the kernel for few rows: with code c and page scale s, the logit takes s_k, and the weight
+// w = 2^(a s_k q.c_k + log2 s_v - M) takes s_v, so both products run on codes, which f16 holds exactly, and the
+// denominator sums w / s_v.  w is kept between 2^7 and 2^15 of its row's largest, as f16 for the second product; sums are
+// f32.  A group of 16 tokens is in one page, so a row pays one product per group for the scales, not one per key.
+//
+// A CTA works on up to 256 rows (tokens x heads of one group) of one request and KV head, as two tiles A and B of 128 rows
+// that share every converted K and V tile of 128 tokens:
+//   warps 0-3, 4-7  softmax of A and of B, one row per thread: the row's q as f16 into shared memory, then per tile the
+//                   maximum, the weights as f16 over the scores they came from in TMEM, the rescaling of O; at the
+//                   end O / sum to the row, or to the workspace
+//   warps 8-11      codes from global memory (the next tile's loads in flight), converted into the 128-byte-swizzled
+//                   layouts of the MMAs: K as rows of dims (K-major), V as rows of tokens (MN-major)
+//   warp 12         issues the MMAs from one thread: S_A S_B | PV_A S_A' | PV_B S_B' | ...: while the tensor cores work
+//                   on one tile's products the other tile's softmax runs
+// TMEM: S_A, S_B (128 columns each; P over the first 64), O_A, O_B.  The tensor pipe runs one thread's MMAs in order, so
+// S' may follow PV into the columns that P is read from, and S' being done means that PV is.
+//
+// Work is dealt out as for few rows: the steps of all (tile pair, head) tasks stand in one line, every CTA takes an equal
+// part, and tasks that this cuts are joined by a second launch.  A first launch lists the tile pairs.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "serving.hpp"
+#include "serving_kv8.cuh"
+#include "tc_common.cuh"
+
+namespace ptowsp::dev {
+
+namespace {
+
+using namespace tc;
+
+constexpr int kRows = 256;               // of a task: two tiles of 128
+constexpr int kKeys = 128;               // per step
+constexpr int kThreads = 13 * 32;
+constexpr int kListThreads = 1024;
+constexpr float kNone = -1.7e38f;        // M before the first visible key
+
+// One pair of row tiles of a request, and the steps before its first one.
+struct Pair {
+    int token0, row0, rows;  // the request's first q token; the pair's first row and its number of rows
+    int base;                // row j's last key: base + (row0 + j) / group
+    int lo, hi;              // keys to walk, lo a multiple of 16
+    int seen;                // the first key that any row sees
+    int units;               // steps per head
+    int64_t before;
+    int request, pad[1];
+};
+static_assert(sizeof(Pair) == 48, "three 16-byte loads");
+
+struct PrefillArgs {
+    AttendArgs a;
+    Pair* pairs;        // the list, in the workspace
+    int64_t* total;     // [0] steps, [1] pairs
+    float* parts;       // two partial results per CTA: [rows][M, l], then [rows][D]
+    int threshold;      // requests with more rows than this are taken
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+// D += A.B for one K = 16 slice, A a shared-memory descriptor (S) or a TMEM address (PV).
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accum) {
+    mma_f16(d, a, b, idesc, accum ? 1u : 0u);
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accum) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accum ? 1u : 0u)
+        : "memory");
+}
+
+// A bounded wait: false when another role gave up or this one does.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
+    uint64_t start = 0;
+    for (uint32_t it = 0;; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((it & 255u) == 255u) {
+            if (*abort_flag) return false;
+            const uint64_t now = globaltimer();
+            if (start == 0) {
+                start = now;
+            } else if (now - start > kTimeoutNs) {
+                if (status) atomicOr(status, PTOWSP_SERVING_TIMEOUT);
+                *abort_flag = 1;
+                return false;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The list of tile pairs
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ int64_t block_inclusive(int64_t v, int64_t* part, int64_t* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t o = __shfl_up_sync(~0u, v, d);
+        if (lane >= d) v += o;
+    }
+    __syncthreads();
+    if (lane == 31) part[warp] = v;
+    __syncthreads();
+    int64_t p = part[lane];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t o = __shfl_up_sync(~0u, p, d);
+        if (lane >= d) p += o;
+    }
+    *total = __shfl_sync(~0u, p, 31);
+    const int64_t before = __shfl_sync(~0u, p, warp ? warp - 1 : 0);
+    return v + (warp ? before : 0);
+}
+
+struct Ask {  // a request as this kernel sees it
+    int token0, nq, len, pairs;
+};
+__device__ __forceinline__ Ask ask_of(const PrefillArgs& g, int r, int* flags) {
+    const AttendArgs& a = g.a;
+    Ask q;
+    q.token0 = a.q_start ? a.q_start[r] : r;
+    q.nq = (a.q_start ? a.q_start[r + 1] : r + 1) - q.token0;
+    if (q.token0 < 0 || q.nq < 0 || q.token0 + static_cast<int64_t>(q.nq) > a.tokens || q.nq > a.max_q) {
+        *flags |= PTOWSP_SERVING_LENGTH;
+        q.nq = 0;
+    }
+    q.len = a.kv_len[r];
+    const int64_t room = static_cast<int64_t>(a.max_pages) << a.cache.page_shift;
+    if (q.len < 0 || q.len > room) {
+        *flags |= PTOWSP_SERVING_LENGTH;
+        q.len = q.len < 0 ? 0 : static_cast<int>(room);
+    }
+    const int64_t rows = static_cast<int64_t>(q.nq) * a.group;
+    q.pairs = rows > g.threshold ? static_cast<int>((rows + kRows - 1) / kRows) : 0;
+    return q;
+}
+
+__global__ void __launch_bounds__(kListThreads) list_kernel(const __grid_constant__ PrefillArgs g, int max_pairs) {
+    __shared__ int64_t part[32];
+    const AttendArgs& a = g.a;
+    int flags = 0;
+    int64_t pairs = 0;
+    // each request's pairs, one thread per request, into their places
+    for (int r0 = 0; r0 < a.requests; r0 += kListThreads) {
+        const int r = r0 + threadIdx.x;
+        Ask q{};
+        if (r < a.requests) q = ask_of(g, r, &flags);
+        int64_t all;
+        const int64_t end = pairs + block_inclusive(q.pairs, part, &all);
+        pairs += all;
+        for (int i = 0; i < q.pairs; ++i) {  // only who they are: the rest is computed in parallel below
+            const int64_t at = end - q.pairs + i;
+            if (at < max_pairs) {
+                g.pairs[at].request = r;
+                g.pairs[at].row0 = i * kRows;
+            }
+        }
+    }
+    if (pairs > max_pairs) {  // the lengths ask for more rows than there are tokens
+        flags |= PTOWSP_SERVING_LENGTH;
+        pairs = max_pairs;
+    }
+    if (flags && a.status) atomicOr(a.status, flags);
+    __syncthreads();
+    int64_t steps = 0;
+    for (int64_t p0 = 0; p0 < pairs; p0 += kListThreads) {
+        const int64_t p = p0 + threadIdx.x;
+        int64_t mine = 0;
+        Pair t{};
+        if (p < pairs) {
+            int ignore = 0;
+            t.request = g.pairs[p].request;
+            t.row0 = g.pairs[p].row0;
+            const Ask q = ask_of(g, t.request, &ignore);
+            t.token0 = q.token0;
+            t.rows = static_cast<int>(min(static_cast<int64_t>(kRows), static_cast<int64_t>(q.nq) * a.group - t.row0));
+            t.base = q.len - q.nq;
+            const int first = t.base + t.row0 / a.group, last = t.base + (t.row0 + t.rows - 1) / a.group;
+            t.hi = max(0, min(q.len, last + 1));
+            if (a.window > 0 && first - a.window + 1 > 0) t.seen = first - a.window + 1;
+            t.lo = t.seen & ~15;
+            t.units = t.hi > t.lo ? (t.hi - t.lo + kKeys - 1) / kKeys : 1;  // a task without keys writes its zeros
+            mine = static_cast<int64_t>(t.units) * a.cache.kv_heads;
+        }
+        int64_t all;
+        const int64_t end = steps + block_inclusive(mine, part, &all);
+        steps += all;
+        if (p < pairs) {
+            t.before = end - mine;
+            g.pairs[p] = t;
+        }
+    }
+    if (threadIdx.x == 0) {
+        g.total[0] = steps;
+        g.total[1] = pairs;
+    }
+}
+
+// The share of CTA c of n in `total` steps.
+__device__ __forceinline__ int64_t share_start(int64_t total, int n, int64_t c) {
+    const int64_t q = total / n, r = total - q * n;
+    return c * q + (c < r ? c : r);
+}
+__device__ __forceinline__ int64_t share_owner(int64_t total, int n, int64_t i) {
+    const int64_t q = total / n, r = total - q * n, big = r * (q + 1);
+    return i < big ? i / (q + 1) : r + (i - big) / q;
+}
+
+// The last pair whose first step is at or before `at`; the whole warp looks.
+__device__ __forceinline__ int find_pair(const Pair* pairs, int n, int64_t at) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, len = n;  // in [lo, lo + len)
+    while (len > 1) {
+        const int stride = (len + 31) / 32;
+        const int i = lo + lane * stride;
+        const bool ok = lane * stride < len && pairs[i].before <= at;
+        const int k = 31 - __clz(static_cast<int>(__ballot_sync(~0u, ok)));
+        lo += k * stride;
+        len = min(stride, len - k * stride);
+    }
+    return lo;
+}
+
+// ---------------------------------------------------------------------------
+// The attention
+// ---------------------------------------------------------------------------
+
+template <int D>
+struct Smem {
+    static constexpr int kBox = 128 * 128;               // 128 rows of 64 f16
+    static constexpr int kBoxes = D / 64;
+    static constexpr int kTile = kBoxes * kBox;
+    static constexpr int kQ = 0;                         // two tiles
+    static constexpr int kK = kQ + 2 * kTile;            // two stages
+    static constexpr int kV = kK + 2 * kTile;            // two stages
+    static constexpr int kScales = kV + 2 * kTile;       // [4][3][8]: k scale, log2 of v scale, 1 / v scale of the groups
+    static constexpr int kBars = kScales + 4 * 3 * 8 * 4;
+    static constexpr int kBytes = kBars + 256 + 1024;    // + alignment to 1024
+};
+static_assert(Smem<128>::kBytes <= 232448, "227 KB of shared memory per CTA");
+
+// The segments of a CTA's share, one after the other; every role walks them alike.
+struct Walk {
+    int64_t at, stop;
+    int pair, head, unit;  // next segment's
+    Pair p;
+    int n;                 // steps of the present segment
+    int unit0, head0;
+    bool whole;
+
+    __device__ bool next(const PrefillArgs& g) {
+        if (at >= stop) return false;
+        p = g.pairs[pair];
+        unit0 = unit;
+        head0 = head;
+        const int64_t left = p.units - unit;
+        n = static_cast<int>(left < stop - at ? left : stop - at);
+        whole = n == p.units;
+        at += n;
+        unit = 0;
+        if (++head == g.a.cache.kv_heads) {
+            head = 0;
+            ++pair;
+        }
+        return true;
+    }
+};
+
+template <int FMT, int D>
+__global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_constant__ PrefillArgs g) {
+    using S = Smem<D>;
+    constexpr int CH = D / 16;               // 16-byte chunks of a row of codes
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const AttendArgs& a = g.a;
+    float* scales = reinterpret_cast<float*>(smem + S::kScales);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
+    const uint32_t bar0 = smem_u32(bars);
+    const uint32_t q_full = bar0, k_full = bar0 + 16, k_empty = bar0 + 32, v_full = bar0 + 48, v_empty = bar0 + 64,
+                   sc_full = bar0 + 80, s_full = bar0 + 112, p_full = bar0 + 128, o_full = bar0 + 144, drain = bar0 + 160;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 21);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
+    __shared__ int first_pair;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const int64_t total = g.total[0];
+    Walk w{};
+    w.at = share_start(total, gridDim.x, blockIdx.x);
+    w.stop = share_start(total, gridDim.x, blockIdx.x + 1);
+    if (w.at >= w.stop) return;  // the whole CTA: nothing is set up yet
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(q_full + 8 * i, 128);
+            mbar_init(k_full + 8 * i, 128);
+            mbar_init(k_empty + 8 * i, 1);
+            mbar_init(v_full + 8 * i, 128);
+            mbar_init(v_empty + 8 * i, 1);
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(p_full + 8 * i, 128);
+            mbar_init(o_full + 8 * i, 1);
+        }
+        for (int i = 0; i < 4; ++i) mbar_init(sc_full + 8 * i, 1);
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        const int p = find_pair(g.pairs, static_cast<int>(g.total[1]), w.at);
+        if (lane == 0) first_pair = p;
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    w.pair = first_pair;
+    {
+        const Pair p = g.pairs[w.pair];
+        const int64_t in = w.at - p.before;
+        w.head = static_cast<int>(in / p.units);
+        w.unit = static_cast<int>(in - static_cast<int64_t>(w.head) * p.units);
+    }
+    const uint32_t sQ = smem_u32(smem + S::kQ), sK = smem_u32(smem + S::kK), sV = smem_u32(smem + S::kV);
+
+    if (warp < 8) {
+        // ---------------- softmax: one row per thread ----------------
+        const int x = warp >> 2;  // tile A or B
+        const int row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_cols = tmem + lanes + x * 128, o_cols = tmem + lanes + 256 + x * 128;
+        uint32_t tiles = 0, steps = 0, segments = 0;  // of this tile; of the CTA; of this tile
+        bool ok = true;
+        while (ok && w.next(g)) {
+            const bool live = w.p.rows > x * 128;  // the whole tile
+            if (!live) {
+                steps += w.n;
+                continue;
+            }
+            const int flat = w.p.row0 + x * 128 + row;
+            const bool real = x * 128 + row < w.p.rows;
+            const int64_t tok = w.p.token0 + flat / a.group;
+            const int hq = w.head0 * a.group + flat % a.group;
+            const int pos = real ? w.p.base + flat / a.group : -1;
+            // -- q as f16 times a power of two that brings the row's largest below 2^15 --
+            float factor;
+            {
+                uint4 raw[D / 8];
+                const uint16_t* src = static_cast<const uint16_t*>(a.q) + tok * a.q_token_stride + hq * a.q_head_stride;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i)
+                    raw[i] = real ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
+                const bool half = a.dtype == PTOWSP_F16;
+                const auto value = [&](uint32_t u, int k) -> float {
+                    if (half) return __half2float(__ushort_as_half(static_cast<unsigned short>(k ? u >> 16 : u & 0xffffu)));
+                    return __uint_as_float(k ? u & 0xffff0000u : u << 16);
+                };
+                float m = 0.f;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) m = fmaxf(m, fmaxf(fabsf(value(u[k], 0)), fabsf(value(u[k], 1))));
+                }
+                int e = 0;
+                if (m > 0.f && m < INFINITY)
+                    e = min(max(14 - (static_cast<int>(__float_as_uint(m) >> 23) - 127), -120), 120);
+                float f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                factor = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                if (a.scale < 0.f) f = -f;  // the factor of the scores stays positive, so a group's maximum is theirs
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                    uint32_t h[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) h[k] = pack2(value(u[k], 0) * f, value(u[k], 1) * f);
+                    *reinterpret_cast<uint4*>(smem + S::kQ + x * S::kTile + (i >> 3) * S::kBox + row * 128 +
+                                              (((i & 7) ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(q_full + 8 * x);
+
+            // steps of this tile that need no mask: every row sees all 128 keys
+            const int first_key = w.p.lo + w.unit0 * kKeys;
+            const int tile_rows = min(128, w.p.rows - x * 128);
+            const int low = w.p.base + (w.p.row0 + x * 128) / a.group;
+            const int high = w.p.base + (w.p.row0 + x * 128 + tile_rows - 1) / a.group;
+            float M = kNone, l = 0.f;
+            for (int j = 0; j < w.n; ++j) {
+                const int key0 = first_key + j * kKeys;
+                const int slot = steps & 3;
+                const bool plain = key0 + kKeys <= min(low + 1, w.p.hi) && (a.window == 0 || key0 > high - a.window);
+                ok = wait_for(sc_full + 8 * slot, (steps >> 2) & 1, abort_flag, a.status) &&
+                     wait_for(s_full + 8 * x, tiles & 1, abort_flag, a.status);
+                ok = __all_sync(~0u, ok);  // the TMEM loads are the whole warp's
+                if (!ok) break;
+                tc_fence_after();
+                ++steps;
+                ++tiles;
+                const float* sc = scales + slot * 24;
+                // columns that the row sees: c0 .. c1
+                const int c1 = min(pos, w.p.hi - 1) - key0, c0 = a.window > 0 ? pos - a.window + 1 - key0 : 0;
+
+                // the largest exponent
+                float top = -INFINITY;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t r[2][32];
+                    tmem_ld32_async(s_cols + h * 64, r[0]);
+                    tmem_ld32_async(s_cols + h * 64 + 32, r[1]);
+                    tmem_wait_ld();
+                    reg_fence(r[0]);
+                    reg_fence(r[1]);
+                    if (!plain) {
+#pragma unroll
+                        for (int c = 0; c < 64; ++c)
+                            if (h * 64 + c > c1 || h * 64 + c < c0) r[c >> 5][c & 31] = 0xff800000u;
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float m = -INFINITY;
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) m = fmaxf(m, __uint_as_float(r[q >> 1][(q & 1) * 16 + c]));
+                        // a group without a page has factor 0 and log2 -inf
+                        top = fmaxf(top, fmaf(m, factor * sc[h * 4 + q], sc[8 + h * 4 + q]));
+                    }
+                }
+                const bool grow = top > M + 15.f;
+                if (__any_sync(~0u, grow)) {
+                    const float m = grow ? top - 7.f : M;
+                    const float f = ex2(M - m);
+                    M = m;
+                    l *= f;
+                    if (j > 0) {  // O holds the steps before this one: PV of step j - 1 came before S of this one
+#pragma unroll 1
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t r[32];
+                            tmem_ld32_async(o_cols + c * 32, r);
+                            tmem_wait_ld();
+                            reg_fence(r);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+                            tmem_st32(o_cols + c * 32, r);
+                        }
+                        tmem_wait_st();
+                    }
+                }
+                // the weights, as f16 over the scores: chunk c's lie in columns that chunks up to c have been read from
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    uint32_t r[32];
+                    tmem_ld32_async(s_cols + h * 32, r);
+                    tmem_wait_ld();
+                    reg_fence(r);
+                    uint32_t p[16];
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const float f = factor * sc[h * 2 + q], c = sc[8 + h * 2 + q] - M;
+                        float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            float w0 = ex2(fmaf(__uint_as_float(r[q * 16 + 2 * i]), f, c));
+                            float w1 = ex2(fmaf(__uint_as_float(r[q * 16 + 2 * i + 1]), f, c));
+                            if (!plain) {
+                                const int col = h * 32 + q * 16 + 2 * i;
+                                if (col > c1 || col < c0) w0 = 0.f;
+                                if (col + 1 > c1 || col + 1 < c0) w1 = 0.f;
+                            }
+                            sum0 += w0;
+                            sum1 += w1;
+                            p[q * 8 + i] = pack2(w0, w1);
+                        }
+                        l = fmaf(sum0 + sum1, sc[16 + h * 2 + q], l);
+                    }
+                    tmem_st16(s_cols + h * 16, p);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(p_full + 8 * x);
+            }
+            if (!ok) break;
+            ok = __all_sync(~0u, wait_for(o_full + 8 * x, segments & 1, abort_flag, a.status));
+            if (!ok) break;
+            ++segments;
+            tc_fence_after();
+            const bool any = l > 0.f || l != l;  // NaN goes through; a row that saw no key is zero
+            const float inv = any ? 1.f / l : 0.f;
+            float* part = g.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (w.unit0 > 0 ? 0 : 1)) * kRows * (D + 2);
+            float* part_o = part + 2 * kRows + (x * 128 + row) * D;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t r[32];
+                tmem_ld32_async(o_cols + c * 32, r);
+                tmem_wait_ld();
+                reg_fence(r);
+                if (!real) continue;
+                if (w.whole) {
+                    uint16_t* to = static_cast<uint16_t*>(a.out) + tok * a.out_token_stride + hq * a.out_head_stride + c * 32;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t h[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float v0 = any ? __uint_as_float(r[i * 8 + 2 * k]) * inv : 0.f;
+                            const float v1 = any ? __uint_as_float(r[i * 8 + 2 * k + 1]) * inv : 0.f;
+                            if (a.dtype == PTOWSP_F16) {
+                                h[k] = pack2(v0, v1);
+                            } else {
+                                const __nv_bfloat162 b = __floats2bfloat162_rn(v0, v1);
+                                h[k] = *reinterpret_cast<const uint32_t*>(&b);
+                            }
+                        }
+                        *reinterpret_cast<uint4*>(to + i * 8) = make_uint4(h[0], h[1], h[2], h[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<uint4*>(part_o + c * 32 + i * 4) =
+                            make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+                }
+            }
+            tc_fence_before();  // O has been read: the next segment's first PV comes after this thread's next P
+            if (real && w.whole) {
+                if (a.lse) a.lse[tok * a.heads + hq] = any ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
+            } else if (real) {
+                part[(x * 128 + row) * 2] = M;
+                part[(x * 128 + row) * 2 + 1] = l;
+            }
+        }
+    } else if (warp < 12) {
+        // ---------------- conversion ----------------
+        constexpr int RPL = 128 / CH;            // rows per load of all 128 threads
+        constexpr int NL = kKeys / RPL;          // loads per tile and thread
+        const int t = threadIdx.x - 8 * 32;
+        const int chunk = t % CH, row0 = t / CH;
+        const int box = chunk >> 2, unit = (chunk & 3) * 2;
+        const int pmask = a.cache.page_size - 1;
+        uint32_t steps = 0;
+        bool ok = true;
+        // page ids of a step's eight groups in lanes 0 .. 7: -1 where no row sees a token
+        const auto ids_of = [&](const Walk& s, int j) -> int {
+            const int tok = s.p.lo + (s.unit0 + j) * kKeys + (lane & 7) * 16;
+            int id = -1;
+            if (tok < s.p.hi && tok + 16 > s.p.seen) {
+                id = a.page_table[s.p.request * a.table_stride + (tok >> a.cache.page_shift)];
+                if (static_cast<uint32_t>(id) >= a.cache.pages) {
+                    id = -1;
+                    if (a.status && t < 8) atomicOr(a.status, PTOWSP_SERVING_PAGE);
+                }
+            }
+            return id;
+        };
+        const auto load = [&](const Kv8Side& side, const Walk& s, int j, int ids, uint4 (&x)[NL]) {
+            const int key0 = s.p.lo + (s.unit0 + j) * kKeys;
+            const uint8_t* base = side.codes + s.head0 * side.head_stride + chunk * 16;
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int row = row0 + i * RPL;
+                const int id = __shfl_sync(~0u, ids, row >> 4);
+                x[i] = make_uint4(0, 0, 0, 0);  // a row that is not there must not be NaN
+                if (id >= 0 && key0 + row < s.p.hi)
+                    x[i] = __ldg(reinterpret_cast<const uint4*>(base + static_cast<int64_t>(id) * side.page_stride +
+                                                                ((key0 + row) & pmask) * side.token_stride));
+            }
+        };
+        // both 16-byte halves of each chunk's f16; the boxes' lanes take them in turn, so that no two meet in a bank
+        const auto store = [&](uint8_t* tile, const uint4 (&x)[NL]) {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int row = row0 + i * RPL;
+                uint32_t h[8];
+                codes_f16<FMT>(x[i].x, h[0], h[1]);
+                codes_f16<FMT>(x[i].y, h[2], h[3]);
+                codes_f16<FMT>(x[i].z, h[4], h[5]);
+                codes_f16<FMT>(x[i].w, h[6], h[7]);
+                uint8_t* to = tile + box * S::kBox + row * 128;
+                const bool swap = box & 1;
+                const int ua = (unit + (swap ? 1 : 0)) ^ (row & 7), ub = (unit + (swap ? 0 : 1)) ^ (row & 7);
+                *reinterpret_cast<uint4*>(to + (ua << 4)) =
+                    swap ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4*>(to + (ub << 4)) =
+                    swap ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]);
+            }
+            fence_proxy_async_smem();
+        };
+        bool more = w.next(g);
+        int ids = more ? ids_of(w, 0) : -1;
+        uint4 kx[NL], vx[NL];
+        load(a.cache.k, w, 0, ids, kx);
+        while (ok && more) {
+            for (int j = 0; ok && j < w.n; ++j) {
+                const int stage = steps & 1, slot = steps & 3;
+                load(a.cache.v, w, j, ids, vx);
+                // the scales of the step: a k scale of 0 and a log2 of -inf hide a group without a page
+                float ks = 0.f, vs = 1.f;
+                if (t < 8 && ids >= 0) {
+                    const int64_t at = static_cast<int64_t>(ids) * a.cache.kv_heads + w.head0;
+                    ks = a.cache.k.scale[at];
+                    vs = a.cache.v.scale[at];
+                }
+                if (steps >= 2)
+                    ok = __all_sync(~0u, wait_for(k_empty + 8 * stage, ((steps >> 1) & 1) ^ 1u, abort_flag, a.status));
+                if (!ok) break;
+                store(smem + S::kK + stage * S::kTile, kx);
+                mbar_arrive(k_full + 8 * stage);
+                if (t < 32) {
+                    if (t < 8) {
+                        const bool there = ids >= 0 && ks > 0.f;
+                        scales[slot * 24 + t] = there ? ks : 0.f;
+                        scales[slot * 24 + 8 + t] = there ? log2f(vs) : -INFINITY;
+                        scales[slot * 24 + 16 + t] = there ? 1.f / vs : 0.f;
+                    }
+                    __syncwarp();
+                    if (t == 0) mbar_arrive(sc_full + 8 * slot);
+                }
+                // the next step's K, perhaps the next segment's
+                Walk n = w;
+                bool go = true;
+                int nj = j + 1;
+                if (nj == w.n) {
+                    go = n.next(g);
+                    nj = 0;
+                }
+                const int next_ids = go ? ids_of(n, nj) : -1;
+                if (go) load(a.cache.k, n, nj, next_ids, kx);
+                if (steps >= 2)
+                    ok = __all_sync(~0u, wait_for(v_empty + 8 * stage, ((steps >> 1) & 1) ^ 1u, abort_flag, a.status));
+                if (!ok) break;
+                store(smem + S::kV + stage * S::kTile, vx);
+                mbar_arrive(v_full + 8 * stage);
+                ids = next_ids;
+                ++steps;
+            }
+            more = w.next(g);
+        }
+    } else if (lane == 0) {
+        // ---------------- MMAs ----------------
+        constexpr uint32_t idesc_s = idesc_f16(128, kKeys, 0), idesc_o = idesc_f16(128, D, 1);
+        const uint64_t q_desc = smem_desc(sQ, 16, 1024), k_desc = smem_desc(sK, 16, 1024);
+        const uint64_t v_desc = smem_desc(sV, S::kBox, 1024);
+        uint32_t steps = 0, seg[2] = {0, 0}, tiles[2] = {0, 0};
+        bool ok = true, issued = false;
+        while (ok && w.next(g)) {
+            const int nx = w.p.rows > 128 ? 2 : 1;
+            const auto scores = [&](int x, uint32_t step) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint64_t off = (k >> 2) * (S::kBox >> 4) + (k & 3) * 2;
+                    mma_ss(tmem + x * 128, q_desc + x * (S::kTile >> 4) + off, k_desc + (step & 1) * (S::kTile >> 4) + off,
+                           idesc_s, k > 0);
+                }
+                mma_commit(s_full + 8 * x);
+                issued = true;
+            };
+            for (int x = 0; ok && x < nx; ++x) {
+                ok = wait_for(q_full + 8 * x, seg[x] & 1, abort_flag, a.status);
+                ++seg[x];
+            }
+            if (ok) ok = wait_for(k_full + 8 * (steps & 1), (steps >> 1) & 1, abort_flag, a.status);
+            if (!ok) break;
+            tc_fence_after();
+            for (int x = 0; x < nx; ++x) scores(x, steps);
+            mma_commit(k_empty + 8 * (steps & 1));
+            for (int j = 0; ok && j < w.n; ++j, ++steps) {
+                const uint32_t stage = steps & 1;
+                const bool last = j + 1 == w.n;
+                for (int x = 0; ok && x < nx; ++x) {
+                    if (x == 0) ok = wait_for(v_full + 8 * stage, (steps >> 1) & 1, abort_flag, a.status);
+                    if (ok) ok = wait_for(p_full + 8 * x, tiles[x] & 1, abort_flag, a.status);
+                    if (!ok) break;
+                    ++tiles[x];
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; ++k)
+                        mma_ts(tmem + 256 + x * 128, tmem + x * 128 + k * 8, v_desc + stage * (S::kTile >> 4) + k * 128,
+                               idesc_o, j > 0 || k > 0);
+                    if (last) mma_commit(o_full + 8 * x);
+                    if (x + 1 == nx) mma_commit(v_empty + 8 * stage);
+                    if (!last) {
+                        if (x == 0) {
+                            ok = wait_for(k_full + 8 * (stage ^ 1), ((steps + 1) >> 1) & 1, abort_flag, a.status);
+                            if (!ok) break;
+                            tc_fence_after();
+                        }
+                        scores(x, steps + 1);
+                        if (x + 1 == nx) mma_commit(k_empty + 8 * (stage ^ 1));
+                    }
+                }
+            }
+        }
+        if (issued) {  // every MMA issued has completed before TMEM is freed
+            mma_commit(drain);
+            const uint64_t start = globaltimer();
+            while (!mbar_try_wait(drain, 0))
+                if (globaltimer() - start > kTimeoutNs) {
+                    if (a.status) atomicOr(a.status, PTOWSP_SERVING_TIMEOUT);
+                    break;
+                }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// ---------------------------------------------------------------------------
+// Joining the tasks that the deal cut: one CTA column per cut, a warp per row, few pieces per task.
+// ---------------------------------------------------------------------------
+
+constexpr int kJoinThreads = 256;
+
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ PrefillArgs g, int ctas) {
+    const AttendArgs& a = g.a;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t total = g.total[0];
+    const int64_t c = blockIdx.x + 1;
+    const int64_t at = share_start(total, ctas, c);
+    if (at >= total) return;
+    const int pair = find_pair(g.pairs, static_cast<int>(g.total[1]), at);
+    const Pair p = g.pairs[pair];
+    const int64_t in = at - p.before;
+    const int head = static_cast<int>(in / p.units);
+    const int64_t begin = p.before + static_cast<int64_t>(head) * p.units, end = begin + p.units;
+    if (at == begin || share_start(total, ctas, c - 1) > begin) return;  // no cut in a task, or not its first one
+    const int pieces = static_cast<int>(share_owner(total, ctas, end - 1) - c) + 2;
+    constexpr int64_t kPiece = static_cast<int64_t>(kRows) * (D + 2);
+    constexpr int V = D / 32;
+    const float* first = g.parts + ((c - 1) * 2 + 1) * kPiece;
+    const auto piece = [&](int i) { return first + (i == 0 ? 0 : (2 * i - 1) * kPiece); };
+    for (int row = blockIdx.y * (kJoinThreads / 32) + warp; row < p.rows; row += gridDim.y * (kJoinThreads / 32)) {
+        float m = kNone;
+        for (int i = lane; i < pieces; i += 32) m = fmaxf(m, piece(i)[row * 2]);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+        float x[V], sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < V; ++k) x[k] = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < pieces; ++i) {
+            const float* o = piece(i);
+            const float li = o[row * 2 + 1];
+            const float f = li == 0.f ? 0.f : ex2(o[row * 2] - m);  // a piece without a key may hold no O
+            sum = fmaf(f, li, sum);
+#pragma unroll
+            for (int k = 0; k < V; ++k) x[k] = f == 0.f ? x[k] : fmaf(f, o[2 * kRows + row * D + lane * V + k], x[k]);
+        }
+        const int flat = p.row0 + row;
+        const int64_t tok = p.token0 + flat / a.group;
+        const int hq = head * a.group + flat % a.group;
+        const bool any = sum > 0.f || sum != sum;
+        const float r = any ? 1.f / sum : 0.f;
+        const int64_t off = tok * a.out_token_stride + hq * a.out_head_stride + lane * V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            if (a.dtype == PTOWSP_F16) static_cast<__half*>(a.out)[off + k] = __float2half_rn(x[k] * r);
+            else static_cast<__nv_bfloat16*>(a.out)[off + k] = __float2bfloat16_rn(x[k] * r);
+        }
+        if (lane == 0 && a.lse) a.lse[tok * a.heads + hq] = any ? (m + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    }
+}
+
+int64_t most_pairs(const AttendArgs& a) {
+    return std::min<int64_t>(a.tokens * a.group / kRows + a.requests,
+                             (static_cast<int64_t>(a.max_q) * a.group + kRows - 1) / kRows * a.requests);
+}
+size_t list_bytes(const AttendArgs& a) { return (256 + static_cast<size_t>(most_pairs(a)) * sizeof(Pair) + 255) / 256 * 256; }
+
+template <int FMT, int D>
+cudaError_t launch(const PrefillArgs& g, int sms, cudaStream_t s) {
+    static SmemOptIn opt_in;
+    cudaError_t e = opt_in.once(reinterpret_cast<const void*>(prefill_kernel<FMT, D>), Smem<D>::kBytes);
+    if (e != cudaSuccess) return e;
+    const int64_t pairs = most_pairs(g.a);
+    if (pairs > INT32_MAX) return cudaErrorInvalidValue;
+    list_kernel<<<1, kListThreads, 0, s>>>(g, static_cast<int>(pairs));
+    prefill_kernel<FMT, D><<<sms, kThreads, Smem<D>::kBytes, s>>>(g);
+    if (sms > 1) join_kernel<D><<<dim3(sms - 1, 8), kJoinThreads, 0, s>>>(g, sms);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t prefill_workspace_bytes(const AttendArgs& a, int sms) {
+    return list_bytes(a) + static_cast<size_t>(sms) * 2 * kRows * (a.cache.head_dim + 2) * sizeof(float);
+}
+
+cudaError_t launch_prefill(const AttendArgs& a, int threshold, char* workspace, int sms, cudaStream_t s) {
+    PrefillArgs g{};
+    g.a = a;
+    g.total = reinterpret_cast<int64_t*>(workspace);
+    g.pairs = reinterpret_cast<Pair*>(workspace + 256);
+    g.parts = reinterpret_cast<float*>(workspace + list_bytes(a));
+    g.threshold = threshold;
+    if (a.cache.format == PTOWSP_KV8_E4M3)
+        return a.cache.head_dim == 64 ? launch<PTOWSP_KV8_E4M3, 64>(g, sms, s) : launch<PTOWSP_KV8_E4M3, 128>(g, sms, s);
+    return a.cache.head_dim == 64 ? launch<PTOWSP_KV8_INT8, 64>(g, sms, s) : launch<PTOWSP_KV8_INT8, 128>(g, sms, s);
+}
+
+}  // namespace ptowsp::dev
