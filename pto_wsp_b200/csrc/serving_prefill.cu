@@ -40,6 +40,7 @@ constexpr int kKeys = 128;               // per step
 constexpr int kThreads = 13 * 32;
 constexpr int kListThreads = 1024;
 constexpr float kNone = -1.7e38f;        // M before the first visible key
+constexpr float kLeast = 1e-30f;         // of a score's factor: positive whatever the scales, and nothing to a finite score
 
 // One pair of row tiles of a request, and the steps before its first one.
 struct Pair {
@@ -71,15 +72,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-
 // D += A.B for one K = 16 slice, A a shared-memory descriptor (S) or a TMEM address (PV).
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accum) {
     mma_f16(d, a, b, idesc, accum ? 1u : 0u);
@@ -395,7 +387,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     e = min(max(14 - (static_cast<int>(__float_as_uint(m) >> 23) - 127), -120), 120);
                 float f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
                 factor = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                if (a.scale < 0.f) f = -f;  // the factor of the scores stays positive, so a group's maximum is theirs
+                // The factor of the scores is positive, so a group's maximum is theirs and a masked score of -inf stays
+                // one: q takes the sign of the scale, or is zero with it.
+                if (a.scale < 0.f) f = -f;
+                if (a.scale == 0.f) f = 0.f;
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) {
                     const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -427,9 +422,21 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 ++steps;
                 ++tiles;
                 const float* sc = scales + slot * 24;
-                // columns that the row sees: c0 .. c1
-                const int c1 = min(pos, w.p.hi - 1) - key0, c0 = a.window > 0 ? pos - a.window + 1 - key0 : 0;
-
+                if (!plain) {  // -inf over what the row does not see
+                    const int c1 = min(pos, w.p.hi - 1) - key0, c0 = a.window > 0 ? pos - a.window + 1 - key0 : 0;
+#pragma unroll 1
+                    for (int h = 0; h < 4; ++h) {
+                        uint32_t r[32];
+                        tmem_ld32_async(s_cols + h * 32, r);
+                        tmem_wait_ld();
+                        reg_fence(r);
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (h * 32 + c > c1 || h * 32 + c < c0) r[c] = 0xff800000u;
+                        tmem_st32(s_cols + h * 32, r);
+                    }
+                    tmem_wait_st();
+                }
                 // the largest exponent
                 float top = -INFINITY;
 #pragma unroll
@@ -440,18 +447,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     tmem_wait_ld();
                     reg_fence(r[0]);
                     reg_fence(r[1]);
-                    if (!plain) {
-#pragma unroll
-                        for (int c = 0; c < 64; ++c)
-                            if (h * 64 + c > c1 || h * 64 + c < c0) r[c >> 5][c & 31] = 0xff800000u;
-                    }
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        float m = -INFINITY;
+                        const uint32_t* v = &r[q >> 1][(q & 1) * 16];
+                        float m0 = __uint_as_float(v[0]), m1 = __uint_as_float(v[1]);
 #pragma unroll
-                        for (int c = 0; c < 16; ++c) m = fmaxf(m, __uint_as_float(r[q >> 1][(q & 1) * 16 + c]));
-                        // a group without a page has factor 0 and log2 -inf
-                        top = fmaxf(top, fmaf(m, factor * sc[h * 4 + q], sc[8 + h * 4 + q]));
+                        for (int c = 2; c < 16; c += 4) {
+                            m0 = fmaxf(fmaxf(m0, __uint_as_float(v[c])), __uint_as_float(v[c + 1]));
+                            if (c + 2 < 16) m1 = fmaxf(fmaxf(m1, __uint_as_float(v[c + 2])), __uint_as_float(v[c + 3]));
+                        }
+                        // a group without a page has a log2 of -inf
+                        top = fmaxf(top, fmaf(fmaxf(m0, m1), fmaxf(factor * sc[h * 4 + q], kLeast), sc[8 + h * 4 + q]));
                     }
                 }
                 const bool grow = top > M + 15.f;
@@ -476,32 +482,30 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 }
                 // the weights, as f16 over the scores: chunk c's lie in columns that chunks up to c have been read from
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    uint32_t r[32];
-                    tmem_ld32_async(s_cols + h * 32, r);
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t r[2][32];
+                    tmem_ld32_async(s_cols + h * 64, r[0]);
+                    tmem_ld32_async(s_cols + h * 64 + 32, r[1]);
                     tmem_wait_ld();
-                    reg_fence(r);
-                    uint32_t p[16];
+                    reg_fence(r[0]);
+                    reg_fence(r[1]);
+                    uint32_t p[32];
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const float f = factor * sc[h * 2 + q], c = sc[8 + h * 2 + q] - M;
+                    for (int q = 0; q < 4; ++q) {
+                        const uint32_t* v = &r[q >> 1][(q & 1) * 16];
+                        const float f = fmaxf(factor * sc[h * 4 + q], kLeast), c = sc[8 + h * 4 + q] - M;
                         float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            float w0 = ex2(fmaf(__uint_as_float(r[q * 16 + 2 * i]), f, c));
-                            float w1 = ex2(fmaf(__uint_as_float(r[q * 16 + 2 * i + 1]), f, c));
-                            if (!plain) {
-                                const int col = h * 32 + q * 16 + 2 * i;
-                                if (col > c1 || col < c0) w0 = 0.f;
-                                if (col + 1 > c1 || col + 1 < c0) w1 = 0.f;
-                            }
+                            const float w0 = ex2(fmaf(__uint_as_float(v[2 * i]), f, c));
+                            const float w1 = ex2(fmaf(__uint_as_float(v[2 * i + 1]), f, c));
                             sum0 += w0;
                             sum1 += w1;
                             p[q * 8 + i] = pack2(w0, w1);
                         }
-                        l = fmaf(sum0 + sum1, sc[16 + h * 2 + q], l);
+                        l = fmaf(sum0 + sum1, sc[16 + h * 4 + q], l);
                     }
-                    tmem_st16(s_cols + h * 16, p);
+                    tmem_st32(s_cols + h * 32, p);
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -566,12 +570,34 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         const int pmask = a.cache.page_size - 1;
         uint32_t steps = 0;
         bool ok = true;
+        // where the loads are: a step of a segment, as far as they need it
+        struct Cursor {
+            int64_t at;
+            int pair, head, unit, units, lo, hi, seen, request;
+            __device__ void fetch(const PrefillArgs& g) {
+                const Pair p = g.pairs[pair];
+                units = p.units;
+                lo = p.lo;
+                hi = p.hi;
+                seen = p.seen;
+                request = p.request;
+            }
+            __device__ void advance(const PrefillArgs& g, int64_t stop) {
+                ++at;
+                if (++unit < units || at >= stop) return;
+                unit = 0;
+                if (++head < g.a.cache.kv_heads) return;
+                head = 0;
+                ++pair;
+                fetch(g);
+            }
+        };
         // page ids of a step's eight groups in lanes 0 .. 7: -1 where no row sees a token
-        const auto ids_of = [&](const Walk& s, int j) -> int {
-            const int tok = s.p.lo + (s.unit0 + j) * kKeys + (lane & 7) * 16;
+        const auto ids_of = [&](const Cursor& c) -> int {
+            const int tok = c.lo + c.unit * kKeys + (lane & 7) * 16;
             int id = -1;
-            if (tok < s.p.hi && tok + 16 > s.p.seen) {
-                id = a.page_table[s.p.request * a.table_stride + (tok >> a.cache.page_shift)];
+            if (c.at < w.stop && tok < c.hi && tok + 16 > c.seen) {
+                id = a.page_table[c.request * a.table_stride + (tok >> a.cache.page_shift)];
                 if (static_cast<uint32_t>(id) >= a.cache.pages) {
                     id = -1;
                     if (a.status && t < 8) atomicOr(a.status, PTOWSP_SERVING_PAGE);
@@ -579,18 +605,22 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             }
             return id;
         };
-        const auto load = [&](const Kv8Side& side, const Walk& s, int j, int ids, uint4 (&x)[NL]) {
-            const int key0 = s.p.lo + (s.unit0 + j) * kKeys;
-            const uint8_t* base = side.codes + s.head0 * side.head_stride + chunk * 16;
+        const auto load = [&](const Kv8Side& side, const Cursor& c, int ids, uint4 (&x)[NL]) {
+            const int key0 = c.lo + c.unit * kKeys;
+            const uint8_t* base = side.codes + c.head * side.head_stride + chunk * 16;
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
                 const int row = row0 + i * RPL;
                 const int id = __shfl_sync(~0u, ids, row >> 4);
                 x[i] = make_uint4(0, 0, 0, 0);  // a row that is not there must not be NaN
-                if (id >= 0 && key0 + row < s.p.hi)
+                if (id >= 0 && key0 + row < c.hi)
                     x[i] = __ldg(reinterpret_cast<const uint4*>(base + static_cast<int64_t>(id) * side.page_stride +
                                                                 ((key0 + row) & pmask) * side.token_stride));
             }
+        };
+        // the scale of group t of a side
+        const auto scale_of = [&](const Kv8Side& side, const Cursor& c, int ids) -> float {
+            return t < 8 && ids >= 0 ? side.scale[static_cast<int64_t>(ids) * a.cache.kv_heads + c.head] : 0.f;
         };
         // both 16-byte halves of each chunk's f16; the boxes' lanes take them in turn, so that no two meet in a bank
         const auto store = [&](uint8_t* tile, const uint4 (&x)[NL]) {
@@ -612,55 +642,56 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             }
             fence_proxy_async_smem();
         };
-        bool more = w.next(g);
-        int ids = more ? ids_of(w, 0) : -1;
+        // A step's codes are asked for one step ahead, its page ids two.
+        Cursor c{w.at, w.pair, w.head, w.unit};
+        c.fetch(g);
+        const int64_t stop = w.stop;
         uint4 kx[NL], vx[NL];
-        load(a.cache.k, w, 0, ids, kx);
-        while (ok && more) {
-            for (int j = 0; ok && j < w.n; ++j) {
-                const int stage = steps & 1, slot = steps & 3;
-                load(a.cache.v, w, j, ids, vx);
-                // the scales of the step: a k scale of 0 and a log2 of -inf hide a group without a page
-                float ks = 0.f, vs = 1.f;
-                if (t < 8 && ids >= 0) {
-                    const int64_t at = static_cast<int64_t>(ids) * a.cache.kv_heads + w.head0;
-                    ks = a.cache.k.scale[at];
-                    vs = a.cache.v.scale[at];
+        float ks, vs;
+        bool there;
+        int ids;
+        {
+            const int ids0 = ids_of(c);
+            load(a.cache.k, c, ids0, kx);
+            load(a.cache.v, c, ids0, vx);
+            ks = scale_of(a.cache.k, c, ids0);
+            vs = scale_of(a.cache.v, c, ids0);
+            there = ids0 >= 0;
+            c.advance(g, stop);
+            ids = ids_of(c);
+        }
+        for (int64_t left = stop - w.at; left > 0; --left, ++steps) {
+            const int stage = steps & 1, slot = steps & 3;
+            if (steps >= 2)
+                ok = __all_sync(~0u, wait_for(k_empty + 8 * stage, ((steps >> 1) & 1) ^ 1u, abort_flag, a.status));
+            if (!ok) break;
+            store(smem + S::kK + stage * S::kTile, kx);
+            mbar_arrive(k_full + 8 * stage);
+            if (t < 32) {
+                if (t < 8) {  // a group without a page: log2 -inf, nothing to the sum
+                    const bool live = there && ks > 0.f;
+                    scales[slot * 24 + t] = live ? ks : 0.f;
+                    scales[slot * 24 + 8 + t] = live ? log2f(vs) : -INFINITY;
+                    scales[slot * 24 + 16 + t] = live ? 1.f / vs : 0.f;
                 }
-                if (steps >= 2)
-                    ok = __all_sync(~0u, wait_for(k_empty + 8 * stage, ((steps >> 1) & 1) ^ 1u, abort_flag, a.status));
-                if (!ok) break;
-                store(smem + S::kK + stage * S::kTile, kx);
-                mbar_arrive(k_full + 8 * stage);
-                if (t < 32) {
-                    if (t < 8) {
-                        const bool there = ids >= 0 && ks > 0.f;
-                        scales[slot * 24 + t] = there ? ks : 0.f;
-                        scales[slot * 24 + 8 + t] = there ? log2f(vs) : -INFINITY;
-                        scales[slot * 24 + 16 + t] = there ? 1.f / vs : 0.f;
-                    }
-                    __syncwarp();
-                    if (t == 0) mbar_arrive(sc_full + 8 * slot);
-                }
-                // the next step's K, perhaps the next segment's
-                Walk n = w;
-                bool go = true;
-                int nj = j + 1;
-                if (nj == w.n) {
-                    go = n.next(g);
-                    nj = 0;
-                }
-                const int next_ids = go ? ids_of(n, nj) : -1;
-                if (go) load(a.cache.k, n, nj, next_ids, kx);
-                if (steps >= 2)
-                    ok = __all_sync(~0u, wait_for(v_empty + 8 * stage, ((steps >> 1) & 1) ^ 1u, abort_flag, a.status));
-                if (!ok) break;
-                store(smem + S::kV + stage * S::kTile, vx);
-                mbar_arrive(v_full + 8 * stage);
-                ids = next_ids;
-                ++steps;
+                __syncwarp();
+                if (t == 0) mbar_arrive(sc_full + 8 * slot);
             }
-            more = w.next(g);
+            load(a.cache.k, c, ids, kx);
+            ks = scale_of(a.cache.k, c, ids);
+            vs = scale_of(a.cache.v, c, ids);
+            there = ids >= 0;
+            Cursor n = c;
+            n.advance(g, stop);
+            const int next_ids = ids_of(n);
+            if (steps >= 2)
+                ok = __all_sync(~0u, wait_for(v_empty + 8 * stage, ((steps >> 1) & 1) ^ 1u, abort_flag, a.status));
+            if (!ok) break;
+            store(smem + S::kV + stage * S::kTile, vx);
+            mbar_arrive(v_full + 8 * stage);
+            load(a.cache.v, c, ids, vx);
+            c = n;
+            ids = next_ids;
         }
     } else if (lane == 0) {
         // ---------------- MMAs ----------------
