@@ -12,7 +12,7 @@
 //                   end O / sum to the row, or to the workspace
 //   warps 8-11      codes from global memory (the next tile's loads in flight), converted into the 128-byte-swizzled
 //                   layouts of the MMAs: K as rows of dims (K-major), V as rows of tokens (MN-major)
-//   warp 12         issues the MMAs from one thread: S_A S_B | PV_A S_A' | PV_B S_B' | ...: while the tensor cores work
+//   warp 12         (of a group whose other warps idle) issues the MMAs from one thread: S_A S_B | PV_A S_A' | PV_B S_B' | ...: while the tensor cores work
 //                   on one tile's products the other tile's softmax runs
 // TMEM: S_A, S_B (128 columns each; P over the first 64), O_A, O_B.  The tensor pipe runs one thread's MMAs in order, so
 // S' may follow PV into the columns that P is read from, and S' being done means that PV is.
@@ -37,7 +37,9 @@ using namespace tc;
 
 constexpr int kRows = 256;               // of a task: two tiles of 128
 constexpr int kKeys = 128;               // per step
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 512;
+// Registers of a thread: 128 at launch, dealt out anew by role (in all 2 * 128 * 176 + 128 * 112 + 128 * 48 = 512 * 128)
+// so that a softmax thread can hold its row of 128 scores.
 constexpr int kListThreads = 1024;
 constexpr float kNone = -1.7e38f;        // M before the first visible key
 constexpr float kLeast = 1e-30f;         // of a score's factor: positive whatever the scales, and nothing to a finite score
@@ -72,16 +74,78 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// D += A.B for one K = 16 slice, A a shared-memory descriptor (S) or a TMEM address (PV).
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accum) {
-    mma_f16(d, a, b, idesc, accum ? 1u : 0u);
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accum) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accum ? 1u : 0u)
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// With its wait: the values may be used at once.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+// S = Q.K^T over D dims: D / 16 MMAs of K = 16 in one asm block, so that the issuing thread spends one addition per
+// operand.  Both are K-major, 128-byte swizzle: +32 bytes per 16 dims, +16 KB per 64 (descriptors count 16 bytes).
+template <int D>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\t"
+        "setp.ne.b32 p, %3, %3;\n\tsetp.eq.b32 q, %3, %3;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, q;\n\t"
+        "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, q;\n\t"
+        "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, q;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc)
+        : "memory");
+    if constexpr (D == 128)
+        asm volatile(
+            "{\n\t.reg .pred q;\n\t.reg .b64 x, y;\n\t"
+            "setp.eq.b32 q, %3, %3;\n\t"
+            "add.s64 x, %1, 1024;\n\tadd.s64 y, %2, 1024;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, q;\n\t"
+            "add.s64 x, %1, 1026;\n\tadd.s64 y, %2, 1026;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, q;\n\t"
+            "add.s64 x, %1, 1028;\n\tadd.s64 y, %2, 1028;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, q;\n\t"
+            "add.s64 x, %1, 1030;\n\tadd.s64 y, %2, 1030;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, q;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc)
+            : "memory");
+}
+// O (+)= P.V over 128 tokens: P from TMEM (two tokens per column, 8 columns per MMA), V MN-major (+2 KB per 16 tokens).
+__device__ __forceinline__ void mma_values(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\t.reg .b32 x;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 q, %4, %4;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "add.u32 x, %1, 8;\n\tadd.s64 y, %2, 128;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t"
+        "add.u32 x, %1, 16;\n\tadd.s64 y, %2, 256;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t"
+        "add.u32 x, %1, 24;\n\tadd.s64 y, %2, 384;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t"
+        "add.u32 x, %1, 32;\n\tadd.s64 y, %2, 512;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t"
+        "add.u32 x, %1, 40;\n\tadd.s64 y, %2, 640;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t"
+        "add.u32 x, %1, 48;\n\tadd.s64 y, %2, 768;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t"
+        "add.u32 x, %1, 56;\n\tadd.s64 y, %2, 896;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accum)
         : "memory");
 }
 
@@ -345,6 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
 
     if (warp < 8) {
         // ---------------- softmax: one row per thread ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
         const int x = warp >> 2;  // tile A or B
         const int row = (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -437,28 +502,25 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     }
                     tmem_wait_st();
                 }
+                uint32_t r[4][32];
+#pragma unroll
+                for (int h = 0; h < 4; ++h) tmem_ld32_async(s_cols + h * 32, r[h]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int h = 0; h < 4; ++h) reg_fence(r[h]);
                 // the largest exponent
                 float top = -INFINITY;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t r[2][32];
-                    tmem_ld32_async(s_cols + h * 64, r[0]);
-                    tmem_ld32_async(s_cols + h * 64 + 32, r[1]);
-                    tmem_wait_ld();
-                    reg_fence(r[0]);
-                    reg_fence(r[1]);
+                for (int q = 0; q < 8; ++q) {
+                    const uint32_t* v = &r[q >> 1][(q & 1) * 16];
+                    float m0 = __uint_as_float(v[0]), m1 = __uint_as_float(v[1]);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const uint32_t* v = &r[q >> 1][(q & 1) * 16];
-                        float m0 = __uint_as_float(v[0]), m1 = __uint_as_float(v[1]);
-#pragma unroll
-                        for (int c = 2; c < 16; c += 4) {
-                            m0 = fmaxf(fmaxf(m0, __uint_as_float(v[c])), __uint_as_float(v[c + 1]));
-                            if (c + 2 < 16) m1 = fmaxf(fmaxf(m1, __uint_as_float(v[c + 2])), __uint_as_float(v[c + 3]));
-                        }
-                        // a group without a page has a log2 of -inf
-                        top = fmaxf(top, fmaf(fmaxf(m0, m1), fmaxf(factor * sc[h * 4 + q], kLeast), sc[8 + h * 4 + q]));
+                    for (int c = 2; c < 16; c += 4) {
+                        m0 = fmaxf(fmaxf(m0, __uint_as_float(v[c])), __uint_as_float(v[c + 1]));
+                        if (c + 2 < 16) m1 = fmaxf(fmaxf(m1, __uint_as_float(v[c + 2])), __uint_as_float(v[c + 3]));
                     }
+                    // a group without a page has a log2 of -inf
+                    top = fmaxf(top, fmaf(fmaxf(m0, m1), fmaxf(factor * sc[q], kLeast), sc[8 + q]));
                 }
                 const bool grow = top > M + 15.f;
                 if (__any_sync(~0u, grow)) {
@@ -468,32 +530,24 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     l *= f;
                     if (j > 0) {  // O holds the steps before this one: PV of step j - 1 came before S of this one
 #pragma unroll 1
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t r[32];
-                            tmem_ld32_async(o_cols + c * 32, r);
-                            tmem_wait_ld();
-                            reg_fence(r);
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_ld16(o_cols + c * 16, o);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
-                            tmem_st32(o_cols + c * 32, r);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st16(o_cols + c * 16, o);
                         }
                         tmem_wait_st();
                     }
                 }
-                // the weights, as f16 over the scores: chunk c's lie in columns that chunks up to c have been read from
+                // the weights, as f16 over the scores
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t r[2][32];
-                    tmem_ld32_async(s_cols + h * 64, r[0]);
-                    tmem_ld32_async(s_cols + h * 64 + 32, r[1]);
-                    tmem_wait_ld();
-                    reg_fence(r[0]);
-                    reg_fence(r[1]);
-                    uint32_t p[32];
+                for (int h = 0; h < 4; ++h) {
+                    uint32_t p[16];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const uint32_t* v = &r[q >> 1][(q & 1) * 16];
-                        const float f = fmaxf(factor * sc[h * 4 + q], kLeast), c = sc[8 + h * 4 + q] - M;
+                    for (int q = 0; q < 2; ++q) {
+                        const uint32_t* v = &r[h][q * 16];
+                        const float f = fmaxf(factor * sc[h * 2 + q], kLeast), c = sc[8 + h * 2 + q] - M;
                         float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
@@ -503,9 +557,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                             sum1 += w1;
                             p[q * 8 + i] = pack2(w0, w1);
                         }
-                        l = fmaf(sum0 + sum1, sc[16 + h * 4 + q], l);
+                        l = fmaf(sum0 + sum1, sc[16 + h * 2 + q], l);
                     }
-                    tmem_st32(s_cols + h * 32, p);
+                    tmem_st16(s_cols + h * 16, p);
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -562,6 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         }
     } else if (warp < 12) {
         // ---------------- conversion ----------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
         constexpr int RPL = 128 / CH;            // rows per load of all 128 threads
         constexpr int NL = kKeys / RPL;          // loads per tile and thread
         const int t = threadIdx.x - 8 * 32;
@@ -605,22 +660,21 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             }
             return id;
         };
-        const auto load = [&](const Kv8Side& side, const Cursor& c, int ids, uint4 (&x)[NL]) {
-            const int key0 = c.lo + c.unit * kKeys;
-            const uint8_t* base = side.codes + c.head * side.head_stride + chunk * 16;
+        const auto load = [&](const Kv8Side& side, int head, int key0, int hi, int ids, uint4 (&x)[NL]) {
+            const uint8_t* base = side.codes + head * side.head_stride + chunk * 16;
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
                 const int row = row0 + i * RPL;
                 const int id = __shfl_sync(~0u, ids, row >> 4);
                 x[i] = make_uint4(0, 0, 0, 0);  // a row that is not there must not be NaN
-                if (id >= 0 && key0 + row < c.hi)
+                if (id >= 0 && key0 + row < hi)
                     x[i] = __ldg(reinterpret_cast<const uint4*>(base + static_cast<int64_t>(id) * side.page_stride +
                                                                 ((key0 + row) & pmask) * side.token_stride));
             }
         };
         // the scale of group t of a side
-        const auto scale_of = [&](const Kv8Side& side, const Cursor& c, int ids) -> float {
-            return t < 8 && ids >= 0 ? side.scale[static_cast<int64_t>(ids) * a.cache.kv_heads + c.head] : 0.f;
+        const auto scale_of = [&](const Kv8Side& side, int head, int ids) -> float {
+            return t < 8 && ids >= 0 ? side.scale[static_cast<int64_t>(ids) * a.cache.kv_heads + head] : 0.f;
         };
         // both 16-byte halves of each chunk's f16; the boxes' lanes take them in turn, so that no two meet in a bank
         const auto store = [&](uint8_t* tile, const uint4 (&x)[NL]) {
@@ -652,10 +706,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         int ids;
         {
             const int ids0 = ids_of(c);
-            load(a.cache.k, c, ids0, kx);
-            load(a.cache.v, c, ids0, vx);
-            ks = scale_of(a.cache.k, c, ids0);
-            vs = scale_of(a.cache.v, c, ids0);
+            load(a.cache.k, c.head, c.lo + c.unit * kKeys, c.hi, ids0, kx);
+            load(a.cache.v, c.head, c.lo + c.unit * kKeys, c.hi, ids0, vx);
+            ks = scale_of(a.cache.k, c.head, ids0);
+            vs = scale_of(a.cache.v, c.head, ids0);
             there = ids0 >= 0;
             c.advance(g, stop);
             ids = ids_of(c);
@@ -677,23 +731,24 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 __syncwarp();
                 if (t == 0) mbar_arrive(sc_full + 8 * slot);
             }
-            load(a.cache.k, c, ids, kx);
-            ks = scale_of(a.cache.k, c, ids);
-            vs = scale_of(a.cache.v, c, ids);
-            there = ids >= 0;
-            Cursor n = c;
-            n.advance(g, stop);
-            const int next_ids = ids_of(n);
+            const int head = c.head, key0 = c.lo + c.unit * kKeys, hi = c.hi, here = ids;
+            load(a.cache.k, head, key0, hi, here, kx);
+            ks = scale_of(a.cache.k, head, here);
+            vs = scale_of(a.cache.v, head, here);
+            there = here >= 0;
+            c.advance(g, stop);
+            ids = ids_of(c);
             if (steps >= 2)
                 ok = __all_sync(~0u, wait_for(v_empty + 8 * stage, ((steps >> 1) & 1) ^ 1u, abort_flag, a.status));
             if (!ok) break;
             store(smem + S::kV + stage * S::kTile, vx);
             mbar_arrive(v_full + 8 * stage);
-            load(a.cache.v, c, ids, vx);
-            c = n;
-            ids = next_ids;
+            load(a.cache.v, head, key0, hi, here, vx);
         }
-    } else if (lane == 0) {
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    }
+    if (warp == 12 && lane == 0) {
         // ---------------- MMAs ----------------
         constexpr uint32_t idesc_s = idesc_f16(128, kKeys, 0), idesc_o = idesc_f16(128, D, 1);
         const uint64_t q_desc = smem_desc(sQ, 16, 1024), k_desc = smem_desc(sK, 16, 1024);
@@ -703,12 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         while (ok && w.next(g)) {
             const int nx = w.p.rows > 128 ? 2 : 1;
             const auto scores = [&](int x, uint32_t step) {
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint64_t off = (k >> 2) * (S::kBox >> 4) + (k & 3) * 2;
-                    mma_ss(tmem + x * 128, q_desc + x * (S::kTile >> 4) + off, k_desc + (step & 1) * (S::kTile >> 4) + off,
-                           idesc_s, k > 0);
-                }
+                mma_scores<D>(tmem + x * 128, q_desc + x * (S::kTile >> 4), k_desc + (step & 1) * (S::kTile >> 4), idesc_s);
                 mma_commit(s_full + 8 * x);
                 issued = true;
             };
@@ -730,10 +780,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     if (!ok) break;
                     ++tiles[x];
                     tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        mma_ts(tmem + 256 + x * 128, tmem + x * 128 + k * 8, v_desc + stage * (S::kTile >> 4) + k * 128,
-                               idesc_o, j > 0 || k > 0);
+                    mma_values(tmem + 256 + x * 128, tmem + x * 128, v_desc + stage * (S::kTile >> 4), idesc_o, j > 0);
                     if (last) mma_commit(o_full + 8 * x);
                     if (x + 1 == nx) mma_commit(v_empty + 8 * stage);
                     if (!last) {
