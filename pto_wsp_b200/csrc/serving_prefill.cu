@@ -149,6 +149,12 @@ __device__ __forceinline__ void mma_values(uint32_t d, uint32_t a, uint64_t b, u
         : "memory");
 }
 
+// One arrival for the warp, after what all its lanes did (arrivals on one barrier go one by one).
+__device__ __forceinline__ void arrive_warp(uint32_t bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
 // A bounded wait: false when another role gave up or this one does.
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
     uint64_t start = 0;
@@ -371,13 +377,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     if (w.at >= w.stop) return;  // the whole CTA: nothing is set up yet
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(q_full + 8 * i, 128);
-            mbar_init(k_full + 8 * i, 128);
+            mbar_init(q_full + 8 * i, 4);
+            mbar_init(k_full + 8 * i, 4);
             mbar_init(k_empty + 8 * i, 1);
-            mbar_init(v_full + 8 * i, 128);
+            mbar_init(v_full + 8 * i, 4);
             mbar_init(v_empty + 8 * i, 1);
             mbar_init(s_full + 8 * i, 1);
-            mbar_init(p_full + 8 * i, 128);
+            mbar_init(p_full + 8 * i, 4);
             mbar_init(o_full + 8 * i, 1);
         }
         for (int i = 0; i < 4; ++i) mbar_init(sc_full + 8 * i, 1);
@@ -467,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 }
             }
             fence_proxy_async_smem();
-            mbar_arrive(q_full + 8 * x);
+            arrive_warp(q_full + 8 * x);
 
             // steps of this tile that need no mask: every row sees all 128 keys
             const int first_key = w.p.lo + w.unit0 * kKeys;
@@ -563,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 }
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(p_full + 8 * x);
+                arrive_warp(p_full + 8 * x);
             }
             if (!ok) break;
             ok = __all_sync(~0u, wait_for(o_full + 8 * x, segments & 1, abort_flag, a.status));
@@ -720,7 +726,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 ok = __all_sync(~0u, wait_for(k_empty + 8 * stage, ((steps >> 1) & 1) ^ 1u, abort_flag, a.status));
             if (!ok) break;
             store(smem + S::kK + stage * S::kTile, kx);
-            mbar_arrive(k_full + 8 * stage);
+            arrive_warp(k_full + 8 * stage);
             if (t < 32) {
                 if (t < 8) {  // a group without a page: log2 -inf, nothing to the sum
                     const bool live = there && ks > 0.f;
@@ -742,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 ok = __all_sync(~0u, wait_for(v_empty + 8 * stage, ((steps >> 1) & 1) ^ 1u, abort_flag, a.status));
             if (!ok) break;
             store(smem + S::kV + stage * S::kTile, vx);
-            mbar_arrive(v_full + 8 * stage);
+            arrive_warp(v_full + 8 * stage);
             load(a.cache.v, head, key0, hi, here, vx);
         }
     } else {
