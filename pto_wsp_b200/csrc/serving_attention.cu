@@ -33,15 +33,6 @@ constexpr float kNone = -1.7e38f;         // M before the first visible key: bel
 // CTAs per SM: with one fragment of q rows 128 registers do, and 16 warps hide each other's latencies
 __host__ __device__ constexpr int ctas_per_sm(int nb) { return nb == 1 ? 4 : nb == 2 ? 3 : 2; }
 
-// A box of a page's codes (D bytes of one head, some tokens) into shared memory; its bytes count on `bar`.
-__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, int head, int token, int page,
-                                              uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-        "[%6];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(head), "r"(token), "r"(page), "r"(bar)
-        : "memory");
-}
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -807,18 +798,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NB)) attend_kernel(const
     asm volatile("griddepcontrol.wait;" ::: "memory");  // on every path: what follows in the stream counts on it
 }
 
-// The codes as a tensor [pages][page_size][heads][D] whose box is one head's D bytes of up to 32 tokens of a page.
-bool page_map(CUtensorMap* m, const Kv8& c, const Kv8Side& side) {
-    const uint64_t dims[4] = {static_cast<uint64_t>(c.head_dim), static_cast<uint64_t>(c.kv_heads),
-                              static_cast<uint64_t>(c.page_size), static_cast<uint64_t>(c.pages)};
-    // a dimension of one element has no stride that matters
-    const uint64_t strides[3] = {c.kv_heads > 1 ? static_cast<uint64_t>(side.head_stride) : dims[0],
-                                 static_cast<uint64_t>(side.token_stride),
-                                 c.pages > 1 ? static_cast<uint64_t>(side.page_stride) : dims[0]};
-    const uint32_t box[4] = {static_cast<uint32_t>(c.head_dim), 1, c.page_size < 32 ? 16u : 32u, 1};
-    return tc::make_map_u8_4d(m, side.codes, dims, strides, box);
-}
-
 // Zeroes the arrival counters.  The attention starts beside it and waits for it before its first arrival.
 __global__ void clear_arrivals(int* counts, int n) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -833,7 +812,9 @@ cudaError_t launch_rows(const AttendArgs& a, int sms, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const int ctas = sms * ctas_per_sm(NB);
     CUtensorMap k_map, v_map;
-    if (!page_map(&k_map, a.cache, a.cache.k) || !page_map(&v_map, a.cache, a.cache.v)) return cudaErrorInvalidValue;
+    const int box = a.cache.page_size < kTile ? a.cache.page_size : kTile;
+    if (!kv8_map(&k_map, a.cache, a.cache.k, box, true) || !kv8_map(&v_map, a.cache, a.cache.v, box, true))
+        return cudaErrorInvalidValue;
     clear_arrivals<<<1, 256, 0, s>>>(reinterpret_cast<int*>(a.workspace), ctas);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
@@ -882,6 +863,17 @@ AttendArgs split(const AttendArgs& a) {
 }
 
 }  // namespace
+
+bool kv8_map(CUtensorMap* m, const Kv8& c, const Kv8Side& side, int tokens, bool swizzle) {
+    const uint64_t dims[4] = {static_cast<uint64_t>(c.head_dim), static_cast<uint64_t>(c.kv_heads),
+                              static_cast<uint64_t>(c.page_size), static_cast<uint64_t>(c.pages)};
+    // a dimension of one element has no stride that matters
+    const uint64_t strides[3] = {c.kv_heads > 1 ? static_cast<uint64_t>(side.head_stride) : dims[0],
+                                 static_cast<uint64_t>(side.token_stride),
+                                 c.pages > 1 ? static_cast<uint64_t>(side.page_stride) : dims[0]};
+    const uint32_t box[4] = {static_cast<uint32_t>(c.head_dim), 1, static_cast<uint32_t>(tokens), 1};
+    return tc::make_map_u8_4d(m, side.codes, dims, strides, box, swizzle);
+}
 
 size_t attend_workspace_bytes(const AttendArgs& args, int sms) {
     const AttendArgs a = split(args);

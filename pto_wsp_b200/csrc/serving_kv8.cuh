@@ -1,13 +1,14 @@
 // Conversions of the 8-bit cache codes, shared by its writer and its readers.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
 
-#include "../../include/ptowsp_cuda.h"
+#include "serving.hpp"
 
 namespace ptowsp::dev {
 
@@ -28,6 +29,20 @@ __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi
         *reinterpret_cast<__half2*>(&hi) = __hsub2(*reinterpret_cast<__half2*>(&hi), bias);
     }
 }
+
+// A box of a page's codes (a head's dims of some tokens) into shared memory; its bytes count on `bar`.
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, int head, int token, int page,
+                                              uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(head), "r"(token), "r"(page), "r"(bar)
+        : "memory");
+}
+
+// Host: one side's codes as a tensor [pages][page_size][heads][head_dim] whose box is one head's dims of `tokens` tokens
+// of a page, with the 64- or 128-byte swizzle of the row's length or none.
+bool kv8_map(CUtensorMap* m, const Kv8& c, const Kv8Side& side, int tokens, bool swizzle);
 
 template <int FMT>
 __device__ __forceinline__ void decode4(uint32_t w, float (&f)[4]) {

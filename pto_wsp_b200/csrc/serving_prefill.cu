@@ -10,8 +10,9 @@
 //   warps 0-3, 4-7  softmax of A and of B, one row per thread: the row's q as f16 into shared memory, then per tile the
 //                   maximum, the weights as f16 over the scores they came from in TMEM, the rescaling of O; at the
 //                   end O / sum to the row, or to the workspace
-//   warps 8-11      codes from global memory (the next tile's loads in flight), converted into the 128-byte-swizzled
-//                   layouts of the MMAs: K as rows of dims (K-major), V as rows of tokens (MN-major)
+//   warps 8-11      codes from the landing place in shared memory, converted into the 128-byte-swizzled layouts of the
+//                   MMAs: K as rows of dims (K-major), V as rows of tokens (MN-major)
+//   warp 13         asks for the codes by TMA, a box per 16 tokens, and gives the groups' scales
 //   warp 12         (of a group whose other warps idle) issues the MMAs from one thread: S_A S_B | PV_A S_A' | PV_B S_B' | ...: while the tensor cores work
 //                   on one tile's products the other tile's softmax runs
 // TMEM: S_A, S_B (128 columns each; P over the first 64), O_A, O_B.  The tensor pipe runs one thread's MMAs in order, so
@@ -38,7 +39,7 @@ using namespace tc;
 constexpr int kRows = 256;               // of a task: two tiles of 128
 constexpr int kKeys = 128;               // per step
 constexpr int kThreads = 512;
-// Registers of a thread: 128 at launch, dealt out anew by role (in all 2 * 128 * 176 + 128 * 112 + 128 * 48 = 512 * 128)
+// Registers of a thread: 128 at launch, dealt out anew by role (in all 2 * 128 * 176 + 128 * 96 + 128 * 64 = 512 * 128)
 // so that a softmax thread can hold its row of 128 scores.
 constexpr int kListThreads = 1024;
 constexpr float kNone = -1.7e38f;        // M before the first visible key
@@ -320,8 +321,10 @@ struct Smem {
     static constexpr int kQ = 0;                         // two tiles
     static constexpr int kK = kQ + 2 * kTile;            // two stages
     static constexpr int kV = kK + 2 * kTile;            // two stages
-    static constexpr int kScales = kV + 2 * kTile;       // [4][3][8]: k scale, log2 of v scale, 1 / v scale of the groups
-    static constexpr int kBars = kScales + 4 * 3 * 8 * 4;
+    static constexpr int kLand = kV + 2 * kTile;         // codes of K, of V as they come: [128][D]
+    static constexpr int kScales = kLand + 2 * kKeys * D;  // [4][3][8]: k scale, log2 of v scale, 1 / v scale of the groups
+    static constexpr int kLive = kScales + 4 * 3 * 8 * 4;  // [2][8]: tokens of a landed group that are there
+    static constexpr int kBars = kLive + 2 * 8 * 4;
     static constexpr int kBytes = kBars + 256 + 1024;    // + alignment to 1024
 };
 static_assert(Smem<128>::kBytes <= 232448, "227 KB of shared memory per CTA");
@@ -354,7 +357,8 @@ struct Walk {
 };
 
 template <int FMT, int D>
-__global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_constant__ PrefillArgs g) {
+__global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_constant__ PrefillArgs g, const __grid_constant__ CUtensorMap k_map,
+                   const __grid_constant__ CUtensorMap v_map) {
     using S = Smem<D>;
     constexpr int CH = D / 16;               // 16-byte chunks of a row of codes
     extern __shared__ uint8_t smem_raw[];
@@ -364,9 +368,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
     const uint32_t bar0 = smem_u32(bars);
     const uint32_t q_full = bar0, k_full = bar0 + 16, k_empty = bar0 + 32, v_full = bar0 + 48, v_empty = bar0 + 64,
-                   sc_full = bar0 + 80, s_full = bar0 + 112, p_full = bar0 + 128, o_full = bar0 + 144, drain = bar0 + 160;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 21);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
+                   sc_full = bar0 + 80, s_full = bar0 + 112, p_full = bar0 + 128, o_full = bar0 + 144, drain = bar0 + 160,
+                   l_full = bar0 + 168, l_empty = bar0 + 184;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 25);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+    volatile int* live = reinterpret_cast<volatile int*>(smem + S::kLive);
     __shared__ int first_pair;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -385,6 +391,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             mbar_init(s_full + 8 * i, 1);
             mbar_init(p_full + 8 * i, 4);
             mbar_init(o_full + 8 * i, 1);
+            mbar_init(l_full + 8 * i, 1);
+            mbar_init(l_empty + 8 * i, 4);
         }
         for (int i = 0; i < 4; ++i) mbar_init(sc_full + 8 * i, 1);
         mbar_init(drain, 1);
@@ -622,137 +630,137 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         }
     } else if (warp < 12) {
         // ---------------- conversion ----------------
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-        constexpr int RPL = 128 / CH;            // rows per load of all 128 threads
-        constexpr int NL = kKeys / RPL;          // loads per tile and thread
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        constexpr int RPL = 128 / CH;            // rows that all 128 threads read at once
+        constexpr int NL = kKeys / RPL;          // reads per tile and thread
         const int t = threadIdx.x - 8 * 32;
         const int chunk = t % CH, row0 = t / CH;
         const int box = chunk >> 2, unit = (chunk & 3) * 2;
-        const int pmask = a.cache.page_size - 1;
-        uint32_t steps = 0;
+        const int steps = static_cast<int>(w.stop - w.at);
         bool ok = true;
-        // where the loads are: a step of a segment, as far as they need it
-        struct Cursor {
-            int64_t at;
-            int pair, head, unit, units, lo, hi, seen, request;
-            __device__ void fetch(const PrefillArgs& g) {
-                const Pair p = g.pairs[pair];
-                units = p.units;
-                lo = p.lo;
-                hi = p.hi;
-                seen = p.seen;
-                request = p.request;
-            }
-            __device__ void advance(const PrefillArgs& g, int64_t stop) {
-                ++at;
-                if (++unit < units || at >= stop) return;
-                unit = 0;
-                if (++head < g.a.cache.kv_heads) return;
-                head = 0;
-                ++pair;
-                fetch(g);
-            }
-        };
-        // page ids of a step's eight groups in lanes 0 .. 7: -1 where no row sees a token
-        const auto ids_of = [&](const Cursor& c) -> int {
-            const int tok = c.lo + c.unit * kKeys + (lane & 7) * 16;
-            int id = -1;
-            if (c.at < w.stop && tok < c.hi && tok + 16 > c.seen) {
-                id = a.page_table[c.request * a.table_stride + (tok >> a.cache.page_shift)];
-                if (static_cast<uint32_t>(id) >= a.cache.pages) {
-                    id = -1;
-                    if (a.status && t < 8) atomicOr(a.status, PTOWSP_SERVING_PAGE);
-                }
-            }
-            return id;
-        };
-        const auto load = [&](const Kv8Side& side, int head, int key0, int hi, int ids, uint4 (&x)[NL]) {
-            const uint8_t* base = side.codes + head * side.head_stride + chunk * 16;
+        // one side's tile of step s from its landing place into its stage
+        const auto convert = [&](int side, int s, uint32_t full, uint32_t empty, uint8_t* tiles) {
+            ok = wait_for(l_full + 8 * side, s & 1, abort_flag, a.status);
+            if (!__all_sync(~0u, ok)) return;
+            uint4 x[NL];
+            const uint8_t* from = smem + S::kLand + side * kKeys * D + row0 * D + chunk * 16;
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
                 const int row = row0 + i * RPL;
-                const int id = __shfl_sync(~0u, ids, row >> 4);
-                x[i] = make_uint4(0, 0, 0, 0);  // a row that is not there must not be NaN
-                if (id >= 0 && key0 + row < hi)
-                    x[i] = __ldg(reinterpret_cast<const uint4*>(base + static_cast<int64_t>(id) * side.page_stride +
-                                                                ((key0 + row) & pmask) * side.token_stride));
+                x[i] = *reinterpret_cast<const uint4*>(from + i * RPL * D);
+                if ((row & 15) >= live[side * 8 + (row >> 4)]) x[i] = make_uint4(0, 0, 0, 0);  // stale codes could be NaN
             }
-        };
-        // the scale of group t of a side
-        const auto scale_of = [&](const Kv8Side& side, int head, int ids) -> float {
-            return t < 8 && ids >= 0 ? side.scale[static_cast<int64_t>(ids) * a.cache.kv_heads + head] : 0.f;
-        };
-        // both 16-byte halves of each chunk's f16; the boxes' lanes take them in turn, so that no two meet in a bank
-        const auto store = [&](uint8_t* tile, const uint4 (&x)[NL]) {
+            arrive_warp(l_empty + 8 * side);
+            if (s >= 2) ok = wait_for(empty + 8 * (s & 1), ((s >> 1) & 1) ^ 1u, abort_flag, a.status);
+            if (!__all_sync(~0u, ok)) return;
+            // both 16-byte halves of a chunk's f16; the boxes' lanes take them in turn, so that no two meet in a bank
+            uint8_t* to = tiles + (s & 1) * S::kTile + box * S::kBox + row0 * 128;
+            const bool swap = box & 1;
+            const int ua = ((unit + (swap ? 1 : 0)) ^ (row0 & 7)) << 4, ub = ((unit + (swap ? 0 : 1)) ^ (row0 & 7)) << 4;
 #pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const int row = row0 + i * RPL;
+            for (int i = 0; i < NL; ++i) {  // RPL is a multiple of 8: the swizzle is the same in every row
                 uint32_t h[8];
                 codes_f16<FMT>(x[i].x, h[0], h[1]);
                 codes_f16<FMT>(x[i].y, h[2], h[3]);
                 codes_f16<FMT>(x[i].z, h[4], h[5]);
                 codes_f16<FMT>(x[i].w, h[6], h[7]);
-                uint8_t* to = tile + box * S::kBox + row * 128;
-                const bool swap = box & 1;
-                const int ua = (unit + (swap ? 1 : 0)) ^ (row & 7), ub = (unit + (swap ? 0 : 1)) ^ (row & 7);
-                *reinterpret_cast<uint4*>(to + (ua << 4)) =
+                *reinterpret_cast<uint4*>(to + i * RPL * 128 + ua) =
                     swap ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]);
-                *reinterpret_cast<uint4*>(to + (ub << 4)) =
+                *reinterpret_cast<uint4*>(to + i * RPL * 128 + ub) =
                     swap ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]);
             }
             fence_proxy_async_smem();
+            arrive_warp(full + 8 * (s & 1));
         };
-        // A step's codes are asked for one step ahead, its page ids two.
-        Cursor c{w.at, w.pair, w.head, w.unit};
-        c.fetch(g);
-        const int64_t stop = w.stop;
-        uint4 kx[NL], vx[NL];
-        float ks, vs;
-        bool there;
-        int ids;
-        {
-            const int ids0 = ids_of(c);
-            load(a.cache.k, c.head, c.lo + c.unit * kKeys, c.hi, ids0, kx);
-            load(a.cache.v, c.head, c.lo + c.unit * kKeys, c.hi, ids0, vx);
-            ks = scale_of(a.cache.k, c.head, ids0);
-            vs = scale_of(a.cache.v, c.head, ids0);
-            there = ids0 >= 0;
-            c.advance(g, stop);
-            ids = ids_of(c);
-        }
-        for (int64_t left = stop - w.at; left > 0; --left, ++steps) {
-            const int stage = steps & 1, slot = steps & 3;
-            if (steps >= 2)
-                ok = __all_sync(~0u, wait_for(k_empty + 8 * stage, ((steps >> 1) & 1) ^ 1u, abort_flag, a.status));
-            if (!ok) break;
-            store(smem + S::kK + stage * S::kTile, kx);
-            arrive_warp(k_full + 8 * stage);
-            if (t < 32) {
-                if (t < 8) {  // a group without a page: log2 -inf, nothing to the sum
-                    const bool live = there && ks > 0.f;
-                    scales[slot * 24 + t] = live ? ks : 0.f;
-                    scales[slot * 24 + 8 + t] = live ? log2f(vs) : -INFINITY;
-                    scales[slot * 24 + 16 + t] = live ? 1.f / vs : 0.f;
-                }
-                __syncwarp();
-                if (t == 0) mbar_arrive(sc_full + 8 * slot);
-            }
-            const int head = c.head, key0 = c.lo + c.unit * kKeys, hi = c.hi, here = ids;
-            load(a.cache.k, head, key0, hi, here, kx);
-            ks = scale_of(a.cache.k, head, here);
-            vs = scale_of(a.cache.v, head, here);
-            there = here >= 0;
-            c.advance(g, stop);
-            ids = ids_of(c);
-            if (steps >= 2)
-                ok = __all_sync(~0u, wait_for(v_empty + 8 * stage, ((steps >> 1) & 1) ^ 1u, abort_flag, a.status));
-            if (!ok) break;
-            store(smem + S::kV + stage * S::kTile, vx);
-            arrive_warp(v_full + 8 * stage);
-            load(a.cache.v, head, key0, hi, here, vx);
+        for (int s = 0; s < steps && __all_sync(~0u, ok); ++s) {
+            convert(0, s, k_full, k_empty, smem + S::kK);
+            if (__all_sync(~0u, ok)) convert(1, s, v_full, v_empty, smem + S::kV);
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    }
+    if (warp == 13) {
+        // ---------------- loads ----------------
+        const int pmask = a.cache.page_size - 1;
+        int64_t pair = w.pair;
+        int head = w.head, unit = w.unit;
+        Pair p = g.pairs[pair];
+        int64_t at = w.at;
+        // group lane & 7 of the present step: its page (-1: no row sees a token) and how many of its tokens are there
+        const auto look = [&](int* tokens) -> int {
+            const int tok = p.lo + unit * kKeys + (lane & 7) * 16;
+            int id = -1;
+            *tokens = 0;
+            if (at < w.stop && tok < p.hi && tok + 16 > p.seen) {
+                id = a.page_table[p.request * a.table_stride + (tok >> a.cache.page_shift)];
+                if (static_cast<uint32_t>(id) >= a.cache.pages) {
+                    id = -1;
+                    if (a.status && lane < 8) atomicOr(a.status, PTOWSP_SERVING_PAGE);
+                } else {
+                    *tokens = min(16, p.hi - tok);
+                }
+            }
+            return id;
+        };
+        const auto scale_of = [&](const Kv8Side& side, int id) -> float {
+            return lane < 8 && id >= 0 ? side.scale[static_cast<int64_t>(id) * a.cache.kv_heads + head] : 0.f;
+        };
+        const int steps = static_cast<int>(w.stop - w.at);
+        bool ok = true;
+        int tokens, id = look(&tokens);
+        float ks = scale_of(a.cache.k, id), vs = scale_of(a.cache.v, id);
+        int asked = 0;
+        for (int s = 0; ok && s < steps; ++s) {
+            const int tok = (p.lo + unit * kKeys + (lane & 7) * 16) & pmask, h = head, here = id, count = tokens;
+            const uint32_t there = __ballot_sync(~0u, lane < 8 && here >= 0);
+            for (int side = 0; side < 2; ++side) {
+                if (s > 0) ok = __all_sync(~0u, wait_for(l_empty + 8 * side, (s - 1) & 1, abort_flag, a.status));
+                if (!ok) break;
+                if (lane < 8) live[side * 8 + lane] = count;
+                __syncwarp();
+                if (lane == 0) mbar_expect_tx(l_full + 8 * side, __popc(there) * 16 * D);
+                __syncwarp();
+                if (lane < 8 && here >= 0)
+                    tma_load_page(sQ - S::kQ + S::kLand + side * kKeys * D + lane * 16 * D, side ? &v_map : &k_map, h, tok,
+                                  here, l_full + 8 * side);
+                asked = 2 * s + side + 1;
+                if (side == 0) {
+                    // slot s & 3 was last read in step s - 4: V of step s - 2 has been converted, for which PV of step
+                    // s - 4 had to be done, and with it both tiles' softmax
+                    const int slot = s & 3;
+                    if (lane < 8) {  // a group without a page: log2 -inf, nothing to the sum
+                        const bool any = here >= 0 && ks > 0.f;
+                        scales[slot * 24 + lane] = any ? ks : 0.f;
+                        scales[slot * 24 + 8 + lane] = any ? log2f(vs) : -INFINITY;
+                        scales[slot * 24 + 16 + lane] = any ? 1.f / vs : 0.f;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sc_full + 8 * slot);
+                    // the next step's page and scales
+                    ++at;
+                    if (++unit == p.units && at < w.stop) {
+                        unit = 0;
+                        if (++head == a.cache.kv_heads) {
+                            head = 0;
+                            p = g.pairs[++pair];
+                        }
+                    }
+                    id = look(&tokens);
+                    ks = scale_of(a.cache.k, id);
+                    vs = scale_of(a.cache.v, id);
+                }
+            }
+        }
+        // every copy asked for has landed before shared memory goes away
+        const uint64_t start = globaltimer();
+        for (int side = 0; side < 2; ++side) {
+            const int fills = (asked + 1 - side) / 2;
+            while (fills > 0 && !mbar_try_wait(l_full + 8 * side, (fills - 1) & 1))
+                if (globaltimer() - start > kTimeoutNs) {
+                    if (a.status) atomicOr(a.status, PTOWSP_SERVING_TIMEOUT);
+                    break;
+                }
+        }
     }
     if (warp == 12 && lane == 0) {
         // ---------------- MMAs ----------------
@@ -887,8 +895,11 @@ cudaError_t launch(const PrefillArgs& g, int sms, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const int64_t pairs = most_pairs(g.a);
     if (pairs > INT32_MAX) return cudaErrorInvalidValue;
+    CUtensorMap k_map, v_map;
+    if (!kv8_map(&k_map, g.a.cache, g.a.cache.k, 16, false) || !kv8_map(&v_map, g.a.cache, g.a.cache.v, 16, false))
+        return cudaErrorInvalidValue;
     list_kernel<<<1, kListThreads, 0, s>>>(g, static_cast<int>(pairs));
-    prefill_kernel<FMT, D><<<sms, kThreads, Smem<D>::kBytes, s>>>(g);
+    prefill_kernel<FMT, D><<<sms, kThreads, Smem<D>::kBytes, s>>>(g, k_map, v_map);
     if (sms > 1) join_kernel<D><<<dim3(sms - 1, 8), kJoinThreads, 0, s>>>(g, sms);
     return cudaGetLastError();
 }

@@ -65,7 +65,7 @@ bool make_map_f32(CUtensorMap* m, const void* base, int64_t pitch, int64_t rows,
 }
 
 bool make_map_u8_4d(CUtensorMap* m, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
-                    const uint32_t (&box)[4]) {
+                    const uint32_t (&box)[4], bool swizzle) {
     EncodeTiledFn fn = encode_fn();
     if (!fn || (box[0] != 64 && box[0] != 128)) return false;
     cuuint64_t d[4], st[3];
@@ -73,7 +73,9 @@ bool make_map_u8_4d(CUtensorMap* m, const void* base, const uint64_t (&dims)[4],
     for (int i = 0; i < 4; ++i) d[i] = dims[i], b[i] = box[i];
     for (int i = 0; i < 3; ++i) st[i] = strides[i];
     return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), d, st, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+              !swizzle ? CU_TENSOR_MAP_SWIZZLE_NONE
+              : box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                             : CU_TENSOR_MAP_SWIZZLE_128B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

@@ -284,8 +284,8 @@ bool make_map_f16_plain(CUtensorMap* m, const void* base, uint64_t inner, uint64
                         uint32_t box_x, uint32_t box_y);
 
 // Host: 4-D tensor of bytes, `dims` elements (innermost first), `strides` in bytes of dimensions 1 .. 3, with the swizzle
-// of the box's inner extent (64 or 128 bytes).
+// of the box's inner extent (64 or 128 bytes) or none.
 bool make_map_u8_4d(CUtensorMap* m, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
-                    const uint32_t (&box)[4]);
+                    const uint32_t (&box)[4], bool swizzle);
 
 }  // namespace ptowsp::dev::tc
