@@ -7,15 +7,17 @@
 //
 // A CTA works on up to 256 rows (tokens x heads of one group) of one request and KV head, as two tiles A and B of 128 rows
 // that share every converted K and V tile of 128 tokens:
-//   warps 0-3, 4-7  softmax of A and of B, one row per thread: the row's q as f16 into shared memory, then per tile the
-//                   maximum, the weights as f16 over the scores they came from in TMEM, the rescaling of O; at the
-//                   end O / sum to the row, or to the workspace
-//   warps 8-11      codes from the landing place in shared memory, converted into the 128-byte-swizzled layouts of the
+//   warps 0-15      softmax, eight warps per tile: a row's two threads take 64 keys each and agree on the maximum through
+//                   shared memory.  The row's q as f16 into shared memory, then per step the maximum, the weights as
+//                   f16 over the scores they came from in TMEM, the rescaling of O; at the end O / sum to the row, or
+//                   to the workspace.  One thread per row took 3500 cycles a step, longer than both tiles' MMAs, and
+//                   nothing of the row's chain -- scores, softmax, product, scores -- overlaps within a tile
+//   warps 16-19     codes from the landing place in shared memory, converted into the 128-byte-swizzled layouts of the
 //                   MMAs: K as rows of dims (K-major), V as rows of tokens (MN-major)
-//   warp 13         asks for the codes by TMA, a box per 16 tokens, and gives the groups' scales
-//   warp 12         (of a group whose other warps idle) issues the MMAs from one thread: S_A S_B | PV_A S_A' | PV_B S_B' | ...: while the tensor cores work
+//   warp 20         issues the MMAs from one thread: S_A S_B | PV_A S_A' | PV_B S_B' | ...: while the tensor cores work
 //                   on one tile's products the other tile's softmax runs
-// TMEM: S_A, S_B (128 columns each; P over the first 64), O_A, O_B.  The tensor pipe runs one thread's MMAs in order, so
+//   warp 21         asks for the codes by TMA, a box per 16 tokens, and gives the groups' scales
+// TMEM: S_A, S_B (128 columns each; P over the first 32 of either half), O_A, O_B.  The tensor pipe runs one thread's MMAs in order, so
 // S' may follow PV into the columns that P is read from, and S' being done means that PV is.
 //
 // Work is dealt out as for few rows: the steps of all (tile pair, head) tasks stand in one line, every CTA takes an equal
@@ -38,9 +40,10 @@ using namespace tc;
 
 constexpr int kRows = 256;               // of a task: two tiles of 128
 constexpr int kKeys = 128;               // per step
-constexpr int kThreads = 512;
-// Registers of a thread: 128 at launch, dealt out anew by role (in all 2 * 128 * 176 + 128 * 96 + 128 * 64 = 512 * 128)
-// so that a softmax thread can hold its row of 128 scores.
+constexpr int kSoftmaxWarps = 16;        // eight per tile: two threads per row
+constexpr int kConvertWarp = kSoftmaxWarps, kMmaWarp = kConvertWarp + 4, kLoadWarp = kMmaWarp + 1;
+constexpr int kThreads = (kMmaWarp + 4) * 32;
+// Registers of a thread: 80 at launch, dealt out anew by role: 4 * 128 * 88 + 128 * 72 + 128 * 56 = 768 * 80.
 constexpr int kListThreads = 1024;
 constexpr float kNone = -1.7e38f;        // M before the first visible key
 constexpr float kLeast = 1e-30f;         // of a score's factor: positive whatever the scales, and nothing to a finite score
@@ -126,7 +129,8 @@ __device__ __forceinline__ void mma_scores(uint32_t d, uint64_t a, uint64_t b, u
             "l"(a), "l"(b), "r"(idesc)
             : "memory");
 }
-// O (+)= P.V over 128 tokens: P from TMEM (two tokens per column, 8 columns per MMA), V MN-major (+2 KB per 16 tokens).
+// O (+)= P.V over 128 tokens: P from TMEM (two tokens per column, 8 columns per MMA, the second 64 tokens 64 columns on),
+// V MN-major (+2 KB per 16 tokens).
 __device__ __forceinline__ void mma_values(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\t.reg .b32 x;\n\t"
@@ -138,13 +142,13 @@ __device__ __forceinline__ void mma_values(uint32_t d, uint32_t a, uint64_t b, u
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t"
         "add.u32 x, %1, 24;\n\tadd.s64 y, %2, 384;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t"
-        "add.u32 x, %1, 32;\n\tadd.s64 y, %2, 512;\n\t"
+        "add.u32 x, %1, 64;\n\tadd.s64 y, %2, 512;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t"
-        "add.u32 x, %1, 40;\n\tadd.s64 y, %2, 640;\n\t"
+        "add.u32 x, %1, 72;\n\tadd.s64 y, %2, 640;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t"
-        "add.u32 x, %1, 48;\n\tadd.s64 y, %2, 768;\n\t"
+        "add.u32 x, %1, 80;\n\tadd.s64 y, %2, 768;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t"
-        "add.u32 x, %1, 56;\n\tadd.s64 y, %2, 896;\n\t"
+        "add.u32 x, %1, 88;\n\tadd.s64 y, %2, 896;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(accum)
         : "memory");
@@ -324,8 +328,9 @@ struct Smem {
     static constexpr int kLand = kV + 2 * kTile;         // codes of K, of V as they come: [128][D]
     static constexpr int kScales = kLand + 2 * kKeys * D;  // [4][3][8]: k scale, log2 of v scale, 1 / v scale of the groups
     static constexpr int kLive = kScales + 4 * 3 * 8 * 4;  // [2][8]: tokens of a landed group that are there
-    static constexpr int kBars = kLive + 2 * 8 * 4;
-    static constexpr int kBytes = kBars + 256 + 1024;    // + alignment to 1024
+    static constexpr int kMeet = kLive + 2 * 8 * 4;      // [2 tiles][2 halves][128]: what a row's threads tell each other
+    static constexpr int kBars = kMeet + 2 * 2 * 128 * 4;
+    static constexpr int kBytes = kBars + 320;           // dynamic shared memory begins at a multiple of 1024
 };
 static_assert(Smem<128>::kBytes <= 232448, "227 KB of shared memory per CTA");
 
@@ -361,8 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                    const __grid_constant__ CUtensorMap v_map) {
     using S = Smem<D>;
     constexpr int CH = D / 16;               // 16-byte chunks of a row of codes
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
     const AttendArgs& a = g.a;
     float* scales = reinterpret_cast<float*>(smem + S::kScales);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
@@ -373,7 +377,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 25);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
     volatile int* live = reinterpret_cast<volatile int*>(smem + S::kLive);
-    __shared__ int first_pair;
+    volatile int* first_pair = reinterpret_cast<volatile int*>(bars + 27);
+    const uint32_t meet_full = bar0 + 224;  // [2][4]: of a tile, by the row's quarter
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     const int64_t total = g.total[0];
@@ -381,29 +386,34 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     w.at = share_start(total, gridDim.x, blockIdx.x);
     w.stop = share_start(total, gridDim.x, blockIdx.x + 1);
     if (w.at >= w.stop) return;  // the whole CTA: nothing is set up yet
+    if (smem_u32(smem) & 1023) {  // the swizzled layouts need it
+        if (threadIdx.x == 0 && a.status) atomicOr(a.status, PTOWSP_SERVING_TIMEOUT);
+        return;
+    }
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(q_full + 8 * i, 4);
+            mbar_init(q_full + 8 * i, 8);
             mbar_init(k_full + 8 * i, 4);
             mbar_init(k_empty + 8 * i, 1);
             mbar_init(v_full + 8 * i, 4);
             mbar_init(v_empty + 8 * i, 1);
             mbar_init(s_full + 8 * i, 1);
-            mbar_init(p_full + 8 * i, 4);
+            mbar_init(p_full + 8 * i, 8);
             mbar_init(o_full + 8 * i, 1);
             mbar_init(l_full + 8 * i, 1);
             mbar_init(l_empty + 8 * i, 4);
         }
         for (int i = 0; i < 4; ++i) mbar_init(sc_full + 8 * i, 1);
+        for (int i = 0; i < 8; ++i) mbar_init(meet_full + 8 * i, 2);
         mbar_init(drain, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
         const int p = find_pair(g.pairs, static_cast<int>(g.total[1]), w.at);
-        if (lane == 0) first_pair = p;
+        if (lane == 0) *first_pair = p;
     }
-    if (warp == 12) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -412,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    w.pair = first_pair;
+    w.pair = *first_pair;
     {
         const Pair p = g.pairs[w.pair];
         const int64_t in = w.at - p.before;
@@ -421,15 +431,25 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     }
     const uint32_t sQ = smem_u32(smem + S::kQ), sK = smem_u32(smem + S::kK), sV = smem_u32(smem + S::kV);
 
-    if (warp < 8) {
-        // ---------------- softmax: one row per thread ----------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-        const int x = warp >> 2;  // tile A or B
+    if (warp < kSoftmaxWarps) {
+        // ---------------- softmax: two threads per row ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+        const int x = warp >> 3;          // tile A or B
+        const int half = warp >> 2 & 1;   // keys 64 half .. 64 half + 63 of a step, and as large a part of the dims
         const int row = (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t s_cols = tmem + lanes + x * 128, o_cols = tmem + lanes + 256 + x * 128;
-        uint32_t tiles = 0, steps = 0, segments = 0;  // of this tile; of the CTA; of this tile
+        const uint32_t s_cols = tmem + lanes + x * 128 + half * 64, o_cols = tmem + lanes + 256 + x * 128 + half * (D / 2);
+        float* mine = reinterpret_cast<float*>(smem + S::kMeet) + (x * 2 + half) * 128 + row;
+        const float* other = reinterpret_cast<float*>(smem + S::kMeet) + (x * 2 + (half ^ 1)) * 128 + row;
+        const uint32_t meet_bar = meet_full + 8 * (x * 4 + (warp & 3));
+        uint32_t tiles = 0, steps = 0, segments = 0, meets = 0;  // of this tile; of the CTA; of this tile; of these warps
         bool ok = true;
+        // waits for the row's other thread; both warps come here alike
+        const auto meet = [&]() {
+            arrive_warp(meet_bar);
+            ok = __all_sync(~0u, wait_for(meet_bar, meets & 1, abort_flag, a.status));
+            ++meets;
+        };
         while (ok && w.next(g)) {
             const bool live = w.p.rows > x * 128;  // the whole tile
             if (!live) {
@@ -444,23 +464,28 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             // -- q as f16 times a power of two that brings the row's largest below 2^15 --
             float factor;
             {
-                uint4 raw[D / 8];
-                const uint16_t* src = static_cast<const uint16_t*>(a.q) + tok * a.q_token_stride + hq * a.q_head_stride;
+                uint4 raw[D / 16];
+                const uint16_t* src = static_cast<const uint16_t*>(a.q) + tok * a.q_token_stride + hq * a.q_head_stride +
+                                      half * (D / 2);
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i)
+                for (int i = 0; i < D / 16; ++i)
                     raw[i] = real ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
-                const bool half = a.dtype == PTOWSP_F16;
+                const bool f16 = a.dtype == PTOWSP_F16;
                 const auto value = [&](uint32_t u, int k) -> float {
-                    if (half) return __half2float(__ushort_as_half(static_cast<unsigned short>(k ? u >> 16 : u & 0xffffu)));
+                    if (f16) return __half2float(__ushort_as_half(static_cast<unsigned short>(k ? u >> 16 : u & 0xffffu)));
                     return __uint_as_float(k ? u & 0xffff0000u : u << 16);
                 };
                 float m = 0.f;
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
+                for (int i = 0; i < D / 16; ++i) {
                     const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) m = fmaxf(m, fmaxf(fabsf(value(u[k], 0)), fabsf(value(u[k], 1))));
                 }
+                *mine = m;
+                meet();
+                if (!ok) break;
+                m = fmaxf(m, *other);
                 int e = 0;
                 if (m > 0.f && m < INFINITY)
                     e = min(max(14 - (static_cast<int>(__float_as_uint(m) >> 23) - 127), -120), 120);
@@ -471,71 +496,77 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 if (a.scale < 0.f) f = -f;
                 if (a.scale == 0.f) f = 0.f;
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
+                for (int i = 0; i < D / 16; ++i) {
                     const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
                     uint32_t h[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) h[k] = pack2(value(u[k], 0) * f, value(u[k], 1) * f);
-                    *reinterpret_cast<uint4*>(smem + S::kQ + x * S::kTile + (i >> 3) * S::kBox + row * 128 +
-                                              (((i & 7) ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    const int unit = half * (D / 16) + i;
+                    *reinterpret_cast<uint4*>(smem + S::kQ + x * S::kTile + (unit >> 3) * S::kBox + row * 128 +
+                                              (((unit & 7) ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
                 }
             }
             fence_proxy_async_smem();
             arrive_warp(q_full + 8 * x);
 
             // steps of this tile that need no mask: every row sees all 128 keys
-            const int first_key = w.p.lo + w.unit0 * kKeys;
             const int tile_rows = min(128, w.p.rows - x * 128);
             const int low = w.p.base + (w.p.row0 + x * 128) / a.group;
             const int high = w.p.base + (w.p.row0 + x * 128 + tile_rows - 1) / a.group;
-            float M = kNone, l = 0.f;
-            for (int j = 0; j < w.n; ++j) {
-                const int key0 = first_key + j * kKeys;
-                const int slot = steps & 3;
+            float M = kNone, l = 0.f;  // l: of this thread's keys
+            int key0 = w.p.lo + w.unit0 * kKeys;
+            for (int j = 0; j < w.n; ++j, key0 += kKeys) {
                 const bool plain = key0 + kKeys <= min(low + 1, w.p.hi) && (a.window == 0 || key0 > high - a.window);
-                ok = wait_for(sc_full + 8 * slot, (steps >> 2) & 1, abort_flag, a.status) &&
+                const float* sc = scales + (steps & 3) * 24 + half * 4;
+                ok = wait_for(sc_full + 8 * (steps & 3), (steps >> 2) & 1, abort_flag, a.status) &&
                      wait_for(s_full + 8 * x, tiles & 1, abort_flag, a.status);
                 ok = __all_sync(~0u, ok);  // the TMEM loads are the whole warp's
                 if (!ok) break;
                 tc_fence_after();
                 ++steps;
                 ++tiles;
-                const float* sc = scales + slot * 24;
                 if (!plain) {  // -inf over what the row does not see
-                    const int c1 = min(pos, w.p.hi - 1) - key0, c0 = a.window > 0 ? pos - a.window + 1 - key0 : 0;
+                    const int c1 = min(pos, w.p.hi - 1) - key0 - half * 64;
+                    const int c0 = a.window > 0 ? pos - a.window + 1 - key0 - half * 64 : -64;
 #pragma unroll 1
                     for (int h = 0; h < 4; ++h) {
-                        uint32_t r[32];
-                        tmem_ld32_async(s_cols + h * 32, r);
-                        tmem_wait_ld();
-                        reg_fence(r);
+                        uint32_t r[16];
+                        tmem_ld16(s_cols + h * 16, r);
 #pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            if (h * 32 + c > c1 || h * 32 + c < c0) r[c] = 0xff800000u;
-                        tmem_st32(s_cols + h * 32, r);
+                        for (int c = 0; c < 16; ++c)
+                            if (h * 16 + c > c1 || h * 16 + c < c0) r[c] = 0xff800000u;
+                        tmem_st16(s_cols + h * 16, r);
                     }
                     tmem_wait_st();
                 }
-                uint32_t r[4][32];
-#pragma unroll
-                for (int h = 0; h < 4; ++h) tmem_ld32_async(s_cols + h * 32, r[h]);
-                tmem_wait_ld();
-#pragma unroll
-                for (int h = 0; h < 4; ++h) reg_fence(r[h]);
                 // the largest exponent
                 float top = -INFINITY;
+                {
+                    uint32_t r[2][32];
+                    tmem_ld32_async(s_cols, r[0]);
+                    tmem_ld32_async(s_cols + 32, r[1]);
+                    tmem_wait_ld();
+                    reg_fence(r[0]);
+                    reg_fence(r[1]);
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const uint32_t* v = &r[q >> 1][(q & 1) * 16];
-                    float m0 = __uint_as_float(v[0]), m1 = __uint_as_float(v[1]);
+                    for (int q = 0; q < 4; ++q) {
+                        const uint32_t* v = &r[q >> 1][(q & 1) * 16];
+                        float m0 = __uint_as_float(v[0]), m1 = __uint_as_float(v[1]);
 #pragma unroll
-                    for (int c = 2; c < 16; c += 4) {
-                        m0 = fmaxf(fmaxf(m0, __uint_as_float(v[c])), __uint_as_float(v[c + 1]));
-                        if (c + 2 < 16) m1 = fmaxf(fmaxf(m1, __uint_as_float(v[c + 2])), __uint_as_float(v[c + 3]));
+                        for (int c = 2; c < 16; c += 4) {
+                            m0 = fmaxf(fmaxf(m0, __uint_as_float(v[c])), __uint_as_float(v[c + 1]));
+                            if (c + 2 < 16) m1 = fmaxf(fmaxf(m1, __uint_as_float(v[c + 2])), __uint_as_float(v[c + 3]));
+                        }
+                        // a group without a page has a log2 of -inf
+                        top = fmaxf(top, fmaf(fmaxf(m0, m1), fmaxf(factor * sc[q], kLeast), sc[8 + q]));
                     }
-                    // a group without a page has a log2 of -inf
-                    top = fmaxf(top, fmaf(fmaxf(m0, m1), fmaxf(factor * sc[q], kLeast), sc[8 + q]));
                 }
+                // What a thread posts here its partner has read before the next time: the next scores wait for PV, and
+                // that for both threads' weights.
+                *mine = top;
+                meet();
+                if (!ok) break;
+                top = fmaxf(top, *other);
                 const bool grow = top > M + 15.f;
                 if (__any_sync(~0u, grow)) {
                     const float m = grow ? top - 7.f : M;
@@ -544,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     l *= f;
                     if (j > 0) {  // O holds the steps before this one: PV of step j - 1 came before S of this one
 #pragma unroll 1
-                        for (int c = 0; c < D / 16; ++c) {
+                        for (int c = 0; c < D / 32; ++c) {
                             uint32_t o[16];
                             tmem_ld16(o_cols + c * 16, o);
 #pragma unroll
@@ -554,13 +585,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                         tmem_wait_st();
                     }
                 }
-                // the weights, as f16 over the scores
+                // the weights, as f16 over the first half of this thread's scores; those of the second half are read
+                // before anything is written over them
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    uint32_t p[16];
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t r[32], p[16];
+                    tmem_ld32_async(s_cols + h * 32, r);
+                    tmem_wait_ld();
+                    reg_fence(r);
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
-                        const uint32_t* v = &r[h][q * 16];
+                        const uint32_t* v = &r[q * 16];
                         const float f = fmaxf(factor * sc[h * 2 + q], kLeast), c = sc[8 + h * 2 + q] - M;
                         float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
@@ -584,19 +619,25 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             if (!ok) break;
             ++segments;
             tc_fence_after();
+            *mine = l;
+            meet();
+            if (!ok) break;
+            l += *other;
+            meet();  // both have read: the next segment's first post may come
+            if (!ok) break;
             const bool any = l > 0.f || l != l;  // NaN goes through; a row that saw no key is zero
             const float inv = any ? 1.f / l : 0.f;
             float* part = g.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (w.unit0 > 0 ? 0 : 1)) * kRows * (D + 2);
-            float* part_o = part + 2 * kRows + (x * 128 + row) * D;
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
+            for (int c = 0; c < D / 64; ++c) {
                 uint32_t r[32];
                 tmem_ld32_async(o_cols + c * 32, r);
                 tmem_wait_ld();
                 reg_fence(r);
                 if (!real) continue;
+                const int dim = half * (D / 2) + c * 32;
                 if (w.whole) {
-                    uint16_t* to = static_cast<uint16_t*>(a.out) + tok * a.out_token_stride + hq * a.out_head_stride + c * 32;
+                    uint16_t* to = static_cast<uint16_t*>(a.out) + tok * a.out_token_stride + hq * a.out_head_stride + dim;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         uint32_t h[4];
@@ -614,26 +655,28 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                         *reinterpret_cast<uint4*>(to + i * 8) = make_uint4(h[0], h[1], h[2], h[3]);
                     }
                 } else {
+                    float* to = part + 2 * kRows + (x * 128 + row) * D + dim;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        *reinterpret_cast<uint4*>(part_o + c * 32 + i * 4) =
-                            make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+                        *reinterpret_cast<uint4*>(to + i * 4) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
                 }
             }
             tc_fence_before();  // O has been read: the next segment's first PV comes after this thread's next P
-            if (real && w.whole) {
-                if (a.lse) a.lse[tok * a.heads + hq] = any ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
-            } else if (real) {
-                part[(x * 128 + row) * 2] = M;
-                part[(x * 128 + row) * 2 + 1] = l;
+            if (real && half == 0) {
+                if (!w.whole) {
+                    part[(x * 128 + row) * 2] = M;
+                    part[(x * 128 + row) * 2 + 1] = l;
+                } else if (a.lse) {
+                    a.lse[tok * a.heads + hq] = any ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
+                }
             }
         }
-    } else if (warp < 12) {
+    } else if (warp < kMmaWarp) {
         // ---------------- conversion ----------------
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         constexpr int RPL = 128 / CH;            // rows that all 128 threads read at once
         constexpr int NL = kKeys / RPL;          // reads per tile and thread
-        const int t = threadIdx.x - 8 * 32;
+        const int t = threadIdx.x - kConvertWarp * 32;
         const int chunk = t % CH, row0 = t / CH;
         const int box = chunk >> 2, unit = (chunk & 3) * 2;
         const int steps = static_cast<int>(w.stop - w.at);
@@ -677,9 +720,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             if (__all_sync(~0u, ok)) convert(1, s, v_full, v_empty, smem + S::kV);
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     }
-    if (warp == 13) {
+    if (warp == kLoadWarp) {
         // ---------------- loads ----------------
         const int pmask = a.cache.page_size - 1;
         int64_t pair = w.pair;
@@ -762,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 }
         }
     }
-    if (warp == 12 && lane == 0) {
+    if (warp == kMmaWarp && lane == 0) {
         // ---------------- MMAs ----------------
         constexpr uint32_t idesc_s = idesc_f16(128, kKeys, 0), idesc_o = idesc_f16(128, D, 1);
         const uint64_t q_desc = smem_desc(sQ, 16, 1024), k_desc = smem_desc(sK, 16, 1024);
@@ -822,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 // ---------------------------------------------------------------------------
