@@ -81,7 +81,7 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 // Dealing out the work.  A request has `tiles` tiles of q rows for each KV head, and every one of these tasks takes
 // `units` steps of kUnit tokens.  The steps of all tasks stand in one line (request, tile, head, step), and CTA c of n
 // takes the c-th n-th of it, so all CTAs read the same amount whatever the lengths are.  A task that this cuts leaves
-// one partial result in each CTA it touches, and the last of these CTAs to finish joins them.
+// one partial result in each CTA it touches; the CTA with the first one writes down what a second launch has to join.
 // ---------------------------------------------------------------------------
 
 struct Request {
@@ -204,18 +204,23 @@ __device__ Place find_place(const AttendArgs& a, const Deal& d, const int64_t* s
     return p;
 }
 
-// The workspace: arrival counters, one per CTA, then two partial results per CTA.
+// The workspace: a record per CTA, then two partial results per CTA.
+struct Cut {      // the task whose first piece is the CTA's last share
+    int pieces;   // 0: there is none
+    int row0, head, row_base, rows;
+    int pad[3];
+};
 constexpr int kMaxSms = 512;
-constexpr size_t kArrivals = kMaxSms * 4 * sizeof(int);
+constexpr size_t kCuts = kMaxSms * 4 * sizeof(Cut);
 // A partial result: [rows][M, l], then [rows][D] of O.
 template <int D, int NB>
 constexpr size_t partial_floats() { return static_cast<size_t>(8 * NB) * (D + 2); }
 
 // Divides V dims of a finished row by its sum and stores them, and the row's lse where `first`.
 template <int V>
-__device__ __forceinline__ void store_row(const AttendArgs& a, const Request& q, int head, int flat, int dim,
+__device__ __forceinline__ void store_row(const AttendArgs& a, int row0, int head, int flat, int dim,
                                           const float (&x)[V], float m, float sum, bool first) {
-    const int64_t tok = q.row0 + flat / a.group;
+    const int64_t tok = row0 + flat / a.group;
     const int hq = head * a.group + flat % a.group;
     const bool any = sum > 0.f || sum != sum;  // NaN goes through; a row that saw no key is zero
     const float r = any ? 1.f / sum : 0.f;
@@ -226,91 +231,6 @@ __device__ __forceinline__ void store_row(const AttendArgs& a, const Request& q,
         else static_cast<__nv_bfloat16*>(a.out)[off + k] = __float2bfloat16_rn(x[k] * r);
     }
     if (first && a.lse) a.lse[tok * a.heads + hq] = any ? (m + log2f(sum)) * 0.6931471805599453f : -INFINITY;
-}
-
-// Joins the `pieces` partial results of a task: `first` is the one that CTA c0 left in its second place, the others
-// stand in the first places of CTA c0 + 1 and on.  Few pieces: a warp per row; many (a long history of one request):
-// the warps share the pieces of four rows at a time, so that enough loads are under way.  `x_smem`: [kWarps][4][D + 1].
-template <int D, int NB>
-__device__ void join_pieces(const AttendArgs& a, const Request& q, int head, int row_base, int rows, const float* first,
-                            int pieces, float* x_smem) {
-    constexpr int ROWS = 8 * NB, V = D / 32, R = 4;
-    constexpr int64_t kPiece = partial_floats<D, NB>();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const auto piece = [&](int i) { return first + (i == 0 ? 0 : (2 * i - 1) * kPiece); };
-    const auto top_of = [&](int row) {
-        float m = kNone;
-        for (int i = lane; i < pieces; i += 32) m = fmaxf(m, __ldcg(piece(i) + row * 2));
-#pragma unroll
-        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-        return m;
-    };
-    if (pieces <= 2 * kWarps) {
-        for (int row = warp; row < rows; row += kWarps) {
-            const float m = top_of(row);
-            float x[V], sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < V; ++k) x[k] = 0.f;
-#pragma unroll 4
-            for (int i = 0; i < pieces; ++i) {
-                const float* o = piece(i);
-                const float f = exp2_approx(__ldcg(o + row * 2) - m);
-                sum = fmaf(f, __ldcg(o + row * 2 + 1), sum);
-#pragma unroll
-                for (int k = 0; k < V; ++k) x[k] = fmaf(f, __ldcg(o + 2 * ROWS + row * D + lane * V + k), x[k]);
-            }
-            store_row<V>(a, q, head, row_base + row, lane * V, x, m, sum, lane == 0);
-        }
-        return;
-    }
-    for (int row0 = 0; row0 < rows; row0 += R) {
-        float m[R], x[R][V], sum[R];
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            m[j] = row0 + j < rows ? top_of(row0 + j) : kNone;
-            sum[j] = 0.f;
-#pragma unroll
-            for (int k = 0; k < V; ++k) x[j][k] = 0.f;
-        }
-#pragma unroll 2
-        for (int i = warp; i < pieces; i += kWarps) {
-            const float* st = piece(i) + row0 * 2;
-            const float* o = piece(i) + 2 * ROWS + row0 * D + lane * V;
-#pragma unroll
-            for (int j = 0; j < R; ++j) {
-                if (row0 + j < rows) {
-                    const float f = exp2_approx(__ldcg(st + j * 2) - m[j]);
-                    sum[j] = fmaf(f, __ldcg(st + j * 2 + 1), sum[j]);
-#pragma unroll
-                    for (int k = 0; k < V; ++k) x[j][k] = fmaf(f, __ldcg(o + j * D + k), x[j][k]);
-                }
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            float* to = x_smem + (warp * R + j) * (D + 1);
-#pragma unroll
-            for (int k = 0; k < V; ++k) to[lane * V + k] = x[j][k];
-            if (lane == 0) to[D] = sum[j];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            if (j != warp || row0 + j >= rows) continue;
-            float y[V], l = 0.f;
-#pragma unroll
-            for (int k = 0; k < V; ++k) y[k] = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float* from = x_smem + (w * R + j) * (D + 1);
-                l += from[D];
-#pragma unroll
-                for (int k = 0; k < V; ++k) y[k] += from[lane * V + k];
-            }
-            store_row<V>(a, q, head, row_base + row0 + j, lane * V, y, m[j], l, lane == 0);
-        }
-    }
 }
 
 template <int D, int NB>
@@ -350,13 +270,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NB)) attend_kernel(const
     __shared__ int64_t sums[kThreads];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t4 = lane & 3;
-    __shared__ int arrived;
+    Cut* cut = reinterpret_cast<Cut*>(a.workspace) + blockIdx.x;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     int flags = 0;
     const Deal deal = deal_out<ROWS>(a, gridDim.x, sums, &flags);
     if (blockIdx.x == 0 && flags && a.status) atomicOr(a.status, flags);
     if (deal.total == 0 || blockIdx.x >= deal.ctas) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (threadIdx.x == 0) cut->pieces = 0;
         return;
     }
     int64_t at = deal.start(blockIdx.x);
@@ -721,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NB)) attend_kernel(const
                 }
             }
         float* o_smem = reinterpret_cast<float*>(smem);
-        float* parts = reinterpret_cast<float*>(a.workspace + kArrivals);
+        float* parts = reinterpret_cast<float*>(a.workspace + kCuts);
         float* part = parts + (static_cast<int64_t>(blockIdx.x) * 2 + (p.unit > 0 ? 0 : 1)) * partial_floats<D, NB>();
         constexpr int DP = D / L::kParts;    // dims at a time
         constexpr int V = DP / 32;           // per lane
@@ -752,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NB)) attend_kernel(const
                     for (int k = 0; k < V; ++k) x[k] = fmaf(f, o_smem[(w * ROWS + row) * L::OP + lane * V + k], x[k]);
                 }
                 if (whole) {
-                    store_row<V>(a, p.q, head, row_base + row, h * DP + lane * V, x, m, sum, h == 0 && lane == 0);
+                    store_row<V>(a, p.q.row0, head, row_base + row, h * DP + lane * V, x, m, sum, h == 0 && lane == 0);
                 } else {
 #pragma unroll
                     for (int k = 0; k < V; ++k) part[2 * ROWS + row * D + h * DP + lane * V + k] = x[k];
@@ -763,23 +684,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NB)) attend_kernel(const
                 }
             }
         }
-        if (!whole) {
-            // the last CTA of the task to come here joins what all of them left
-            const int64_t begin = at - p.unit;
-            const int64_t c0 = deal.owner(begin);
-            const int pieces = static_cast<int>(deal.owner(begin + p.q.units - 1) - c0) + 1;
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                asm volatile("griddepcontrol.wait;" ::: "memory");  // the counters are zero from here on
-                arrived = atomicAdd(reinterpret_cast<int*>(a.workspace) + c0, 1);
+        if (at + take == stop && threadIdx.x == 0) {  // the share ends here: is this the first piece of a cut task?
+            Cut c{};
+            if (!whole && p.unit == 0) {
+                c.pieces = static_cast<int>(deal.owner(at + p.q.units - 1)) - static_cast<int>(blockIdx.x) + 1;
+                c.row0 = p.q.row0;
+                c.head = head;
+                c.row_base = row_base;
+                c.rows = rows;
             }
-            __syncthreads();
-            if (arrived == pieces - 1) {
-                __threadfence();
-                join_pieces<D, NB>(a, p.q, head, row_base, rows, parts + (c0 * 2 + 1) * partial_floats<D, NB>(), pieces,
-                                   o_smem);
-            }
+            *cut = c;
         }
         tc::fence_proxy_async_smem();  // what was written to the ring here is ordered before the next share's copies
         __syncthreads();
@@ -795,13 +709,61 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NB)) attend_kernel(const
             }
         }
     }
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // on every path: what follows in the stream counts on it
 }
 
-// Zeroes the arrival counters.  The attention starts beside it and waits for it before its first arrival.
-__global__ void clear_arrivals(int* counts, int n) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    for (int i = threadIdx.x; i < n; i += blockDim.x) counts[i] = 0;
+// Joins the pieces of the tasks that the deal cut: CTA (c, y) those of the task that CTA c wrote down, the second place
+// of c and the first ones of the CTAs behind it.  Few pieces: y = 0 takes all rows, a warp each; many (a long history of
+// one request): four rows per CTA and two warps per row, so that enough loads are under way.
+constexpr int kJoinWarps = 8;
+template <int D, int NB>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ AttendArgs a) {
+    constexpr int ROWS = 8 * NB, V = D / 32;
+    constexpr int64_t kPiece = partial_floats<D, NB>();
+    __shared__ float x_smem[kJoinWarps][D + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Cut cut = reinterpret_cast<const Cut*>(a.workspace)[blockIdx.x];
+    const int pieces = cut.pieces;
+    if (pieces == 0) return;
+    const float* first =
+        reinterpret_cast<const float*>(a.workspace + kCuts) + (static_cast<int64_t>(blockIdx.x) * 2 + 1) * kPiece;
+    const auto piece = [&](int i) { return first + (i == 0 ? 0 : (2 * i - 1) * kPiece); };
+    const bool shared = pieces > 2 * kJoinWarps;
+    if (!shared && blockIdx.y > 0) return;
+    const int step = shared ? 4 * gridDim.y : kJoinWarps;
+    for (int row0 = shared ? blockIdx.y * 4 : 0; row0 < cut.rows; row0 += step) {
+        const int row = row0 + (shared ? warp >> 1 : warp), part = shared ? warp & 1 : 0;
+        const bool real = row < cut.rows;
+        float m = kNone, x[V], sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < V; ++k) x[k] = 0.f;
+        if (real) {
+            for (int i = lane; i < pieces; i += 32) m = fmaxf(m, __ldcg(piece(i) + row * 2));
+#pragma unroll
+            for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+#pragma unroll 8
+            for (int i = part; i < pieces; i += shared ? 2 : 1) {
+                const float* o = piece(i);
+                const float f = exp2_approx(__ldcg(o + row * 2) - m);
+                sum = fmaf(f, __ldcg(o + row * 2 + 1), sum);
+#pragma unroll
+                for (int k = 0; k < V; ++k) x[k] = fmaf(f, __ldcg(o + 2 * ROWS + row * D + lane * V + k), x[k]);
+            }
+        }
+        if (shared) {
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < V; ++k) x_smem[warp][lane * V + k] = x[k];
+            if (lane == 0) x_smem[warp][D] = sum;
+            __syncthreads();
+            if (part == 0) {
+                sum += x_smem[warp + 1][D];
+#pragma unroll
+                for (int k = 0; k < V; ++k) x[k] += x_smem[warp + 1][lane * V + k];
+            }
+        }
+        if (real && part == 0) store_row<V>(a, cut.row0, cut.head, cut.row_base + row, lane * V, x, m, sum, lane == 0);
+    }
 }
 
 template <int FMT, int D, int NB>
@@ -815,20 +777,20 @@ cudaError_t launch_rows(const AttendArgs& a, int sms, cudaStream_t s) {
     const int box = a.cache.page_size < kTile ? a.cache.page_size : kTile;
     if (!kv8_map(&k_map, a.cache, a.cache.k, box, true) || !kv8_map(&v_map, a.cache, a.cache.v, box, true))
         return cudaErrorInvalidValue;
-    clear_arrivals<<<1, 256, 0, s>>>(reinterpret_cast<int*>(a.workspace), ctas);
+    attend_kernel<FMT, D, NB><<<ctas, kThreads, smem, s>>>(a, k_map, v_map);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
+    // the join's CTAs come in as the last ones leave, and wait for them before they read
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.gridDim = dim3(ctas, 2);
+    cfg.blockDim = dim3(kJoinWarps * 32);
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attend_kernel<FMT, D, NB>, a, k_map, v_map);
+    return cudaLaunchKernelEx(&cfg, join_kernel<D, NB>, a);
 }
 
 // Fragments of 8 q rows per tile.  With requests left to the other kernel most of the rest have one token.
@@ -852,7 +814,7 @@ constexpr int kFew = 32;
 
 size_t few_bytes(const AttendArgs& a, int sms) {
     const int nb = fragments(a);
-    return (kArrivals + static_cast<size_t>(sms) * ctas_per_sm(nb) * 2 * (8 * nb) * (a.cache.head_dim + 2) * sizeof(float) +
+    return (kCuts + static_cast<size_t>(sms) * ctas_per_sm(nb) * 2 * (8 * nb) * (a.cache.head_dim + 2) * sizeof(float) +
             255) / 256 * 256;
 }
 
