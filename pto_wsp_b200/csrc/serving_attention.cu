@@ -30,8 +30,9 @@ constexpr int kSlots = 3;                  // tiles of K or V that a warp's ring
 constexpr int kThreads = kWarps * 32;
 constexpr float kNone = -1.7e38f;         // M before the first visible key: below every exponent, yet finite
 
-// CTAs per SM: with one fragment of q rows 128 registers do, and 16 warps hide each other's latencies
-__host__ __device__ constexpr int ctas_per_sm(int nb) { return nb == 1 ? 4 : nb == 2 ? 3 : 2; }
+// CTAs per SM.  With one fragment of q rows four (128 registers) spill: 120 us against 109 over the 64-request decode
+// workload; rings of four tiles instead of three took 112.
+__host__ __device__ constexpr int ctas_per_sm(int nb) { return nb <= 2 ? 3 : 2; }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
