@@ -30,6 +30,7 @@ constexpr int kList = 256;      // elements that are ranked by comparing all pai
 constexpr int kMaxCluster = 8;  // the portable size
 constexpr float kReach = 28.f;  // e^-28 < 2^-40: what is further below the maximum weighs nothing
 constexpr float kBinsPerUnit = kBins / kReach;
+constexpr float kSmallest = 9.094947e-13f;  // 2^-40
 
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
@@ -69,6 +70,7 @@ struct Board {
     int64_t mass[3];
     int count[3];
     uint64_t low, high;
+    int64_t above;
     int listed;
 };
 
@@ -80,6 +82,7 @@ struct Shared {
     uint64_t cut;
     int bin;
     int64_t before;
+    int first_bin, last_bin, near;
 };
 // only where a cut may be looked for
 struct SharedCut {
@@ -174,12 +177,15 @@ struct Row {
     }
 
     // Masses of the warps' regions, and the cluster's mass and count of candidates.
-    __device__ void weigh_regions(int step, int64_t* mass, int* count) {
+    // COUNT: also the candidates' histogram of counts, over cleared bins; false where the row does not take that pass.
+    template <bool COUNT>
+    __device__ bool weigh_regions(int step, int64_t* mass, int* count) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         const int size = region_size(), end = min(n, (warp + 1) * size);
         int64_t m = 0;
         int k = 0;
-        if (inv != 0.f && top < INFINITY && !(CUTS && (cut || raised))) {
+        const bool open = inv != 0.f && top < INFINITY && !(CUTS && (cut || raised));
+        if (open) {
             // The whole row, with no branch: the weight of -inf or NaN comes out as NaN and is none, what is out of reach
             // has no whole part.  w * 2^40 is taken in two parts of 20 bits: adding 2^23 with rounding towards zero
             // leaves floor(w * 2^20) in the low bits, and the rest of the product is exact.  A thread's parts sum to
@@ -187,14 +193,16 @@ struct Row {
             uint32_t hi = 0, lo = 0;
 #pragma unroll 4
             for (int i = warp * size + lane; i < end; i += 32) {
-                float w = expf(distance(as_float(x[i])));
+                const float d = distance(as_float(x[i]));
+                float w = expf(d);
                 w = w >= min_p ? w : 0.f;
                 const float h = __fmaf_rz(w, 1048576.f, 8388608.f);
                 const float rest = fmaf(w, 1048576.f, 8388608.f - h);
                 const float l = __fmaf_rz(rest, 1048576.f, 8388608.f);
                 hi += __float_as_uint(h) - 0x4b000000u;
                 lo += __float_as_uint(l) - 0x4b000000u;
-                if (CUTS) k += w >= 9.094947e-13f;
+                if (CUTS) k += w >= kSmallest;
+                if (COUNT && w >= kSmallest) atomicAdd(&cuts->hist[0][bin_at(d)], 1u);
             }
             m = (static_cast<int64_t>(hi) << 20) + lo;
         } else {
@@ -235,6 +243,7 @@ struct Row {
             *mass += b->mass[step];
             *count += b->count[step];
         }
+        return open;
     }
     __device__ int region_size() const { return ((n + kWarps - 1) / kWarps + 31) & ~31; }
 
@@ -399,24 +408,93 @@ struct Row {
         __syncthreads();
     }
 
-    // Raises `low` to a logit above which the measure of the candidates is sure to reach `target`, because that of the
-    // threads' own largest ones alone does.  The likely tokens are few and mostly in shares of different threads, so few
-    // others are left above it, whatever the vocabulary's size.
-    template <bool MASS>
-    __device__ void raise_low(int64_t target, float own_top) {
-        if (!MASS && target > CL * kThreads / 2) return;
+    // Raises `low` to a logit that at least k candidates reach, because so many of the threads' own largest ones do.  The
+    // likely tokens are few and mostly in shares of different threads, so few others are left above it, whatever the
+    // vocabulary's size.
+    __device__ void raise_low(int k, float own_top) {
+        if (k > CL * kThreads / 2) return;
         clear_bins();
-        if (!(own_top < low)) {
-            // of a cut's ties it counts as the last, whichever it is
-            const int64_t w = MASS ? weigh(own_top, -1 - first) : 1;
-            if (w > 0) count_in<MASS>(bin_of(own_top), w);
+        if (!(own_top < low)) count_in<false>(bin_of(own_top), 1);
+        find_bin<false>(0, k);
+        if (sh.bin >= 0 && sh.bin < kBins - 1) drop_behind(sh.bin);
+    }
+    // Candidates are in the bins up to this one: `low` at its far edge, and a little more for the roundings.
+    __device__ void drop_behind(int bin) {
+        low = fmaxf(low, top - t * ((bin + 1) * (kReach / kBins) * 1.0001f));
+        raised = true;
+    }
+
+    // The bins in which the running mass can reach `limit`, from the counts: a bin's weights lie between those of its
+    // edges.  sh.first_bin, sh.last_bin, and sh.near candidates in the bins up to that.
+    __device__ void window(int64_t limit) {
+        if (threadIdx.x == 0) {
+            sh.last_bin = kBins - 1;
+            sh.near = INT32_MAX;
         }
-        find_bin<MASS>(0, target);
-        // the bin's far edge, and a little more for the roundings
-        if (sh.bin >= 0 && sh.bin < kBins - 1) {
-            low = fmaxf(low, top - t * ((sh.bin + 1) * (kReach / kBins) * 1.0001f));
-            raised = true;
+        uint32_t c0 = 0, c1 = 0;
+#pragma unroll
+        for (int r = 0; r < CL; ++r) {
+            const uint2 k = reinterpret_cast<const uint2*>(of(cuts->hist[0], r))[threadIdx.x];
+            c0 += k.x;
+            c1 += k.y;
         }
+        const int b = 2 * threadIdx.x;
+        const float e0 = expf(-b / kBinsPerUnit), e1 = expf(-(b + 1) / kBinsPerUnit), e2 = expf(-(b + 2) / kBinsPerUnit);
+        // with room for the roundings of the bins and of the weights
+        const auto above = [](float e) { return whole_of(fminf(e * 1.0001f, 1.f)) + 1; };
+        const auto below = [](float e) { return whole_of(e * 0.9999f); };
+        const int64_t u0 = c0 * above(e0), u1 = c1 * above(e1);
+        const int64_t l0 = c0 * below(e1), l1 = b + 2 < kBins ? c1 * below(e2) : 0;  // the last bin has no far edge
+        const int64_t ue = block_inclusive(u0 + u1, sh.part), le = block_inclusive(l0 + l1, sh.part);
+        const int64_t ce = block_inclusive(c0 + c1, sh.part);
+        if (ue >= limit && ue - u0 - u1 < limit) sh.first_bin = ue - u1 >= limit ? b : b + 1;
+        if (le >= limit && le - l0 - l1 < limit) {
+            const bool one = le - l1 >= limit;
+            sh.last_bin = one ? b : b + 1;
+            sh.near = static_cast<int>(one ? ce - c1 : ce);
+        }
+        __syncthreads();
+    }
+
+    // The cut at mass `limit` (less than all) from the counts of weigh_regions<true>: only the weights in front of the
+    // window are summed, and only those inside it go into a histogram, of as many bins over the window.  False where
+    // that leaves too many alike.
+    __device__ bool window_cut(int64_t limit) {
+        const int b0 = sh.first_bin, b1 = sh.last_bin;
+        const float fine = static_cast<float>(kBins) / (b1 - b0 + 1);
+        clear_bins();
+        // -1: in front of the window or not in it; the candidate's weight where it is in or before it
+        const auto place = [&](float v, int i, int64_t* w) -> int {
+            const float d = any_distance(v);
+            const int b = bin_at(d);
+            if (b > b1) {
+                *w = 0;
+                return -1;
+            }
+            *w = weigh(v, i, d);
+            return b < b0 ? -1 : min(kBins - 1, static_cast<int>((-d * kBinsPerUnit - b0) * fine));
+        };
+        int64_t front = 0;
+        each([&](float v, int i) {
+            int64_t w;
+            const int b = place(v, i, &w);
+            if (b < 0) front += w;
+            else if (w > 0) count_in<true>(b, w);
+        });
+        front = block_reduce<int64_t>(front, [](int64_t p, int64_t q) { return p + q; }, sh.part);
+        if (threadIdx.x == 0) sh.board.above = front;
+        sync();
+        front = 0;
+#pragma unroll
+        for (int r = 0; r < CL; ++r) front += of(&sh.board, r)->above;
+        find_bin<true>(front, limit);
+        const int bin = sh.bin;
+        const int64_t before = sh.before;
+        if (bin < 0) return false;
+        const int total = list(false, [&](float v, int i, int64_t* w) { return place(v, i, w) == bin && *w > 0; });
+        if (total > kList) return false;
+        rank_list<true>(before, limit, total);
+        return true;
     }
 
     // Finds the element at which the measure of the candidates, in falling order, reaches `target` (>= 1, at most the
@@ -566,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) sample_kernel(SampleAr
             return true;
         };
         if (k > 0) {
-            row.template raise_low<false>(k, own_top);
+            row.raise_low(k, own_top);
             const int total = row.list(true, weighed);
             if (total <= kList) {
                 row.finish_list(a, r, rank, total, k, top_p, 0);
@@ -586,28 +664,38 @@ __global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) sample_kernel(SampleAr
                 row.low = fmaxf(row.low, value_of(static_cast<uint32_t>(row.cut >> 32)));
             }
         }
-        row.weigh_regions(0, &mass, &count);
-        if (top_p < 1.f) {
-            const int64_t limit = row.limit_of(top_p, mass);
-            if (limit < mass) {
-                const float reach = row.low;
-                row.template raise_low<true>(limit, own_top);
-                if (row.low > reach || a.vocab <= kList) {
+        bool counted = false;
+        if (top_p < 1.f && !row.raised) {
+            row.clear_bins();
+            counted = row.template weigh_regions<true>(0, &mass, &count);
+        } else {
+            row.template weigh_regions<false>(0, &mass, &count);
+        }
+        const int64_t limit = row.limit_of(top_p, mass);
+        if (top_p < 1.f && limit < mass) {
+            bool found = false;
+            if (counted) {
+                row.window(limit);
+                if (sh.near <= kList && sh.last_bin < kBins - 1) {
+                    row.drop_behind(sh.last_bin);
                     const int total = row.list(true, weighed);
                     if (total <= kList) {
                         row.finish_list(a, r, rank, total, 0, top_p, limit);
                         return;
                     }
                 }
+                found = row.window_cut(limit);
+            }
+            if (!found) {
                 // weights below (1 - p) mass / (2 count) are together less than what stays out
                 const double least = 0.5 * (1.0 - static_cast<double>(top_p)) * static_cast<double>(mass) / count;
                 row.template find_cut<true>(limit, static_cast<int64_t>(fmax(least, 0.0)));
-                row.low = fmaxf(row.low, value_of(static_cast<uint32_t>(row.cut >> 32)));
-                row.weigh_regions(1, &mass, &count);
             }
+            row.low = fmaxf(row.low, value_of(static_cast<uint32_t>(row.cut >> 32)));
+            row.template weigh_regions<false>(1, &mass, &count);
         }
     } else {
-        row.weigh_regions(0, &mass, &count);
+        row.template weigh_regions<false>(0, &mass, &count);
     }
 
     // -- the pick: the CTA, then the warp's region, then the element --
