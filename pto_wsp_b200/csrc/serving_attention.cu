@@ -515,6 +515,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NB)) attend_kernel(const
                     }
                 }
             }
+            tc::fence_proxy_async_smem();  // reads that are still queued come before the copy's writes
             __syncwarp();
             ask(&v_map, i + 1, ids1, kslot);  // K's place is free
 
@@ -611,6 +612,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NB)) attend_kernel(const
                     }
                 }
             }
+            tc::fence_proxy_async_smem();
             __syncwarp();
             ask(&k_map, i + 2, ids2, vslot);  // V's place is free
             ids1 = ids2;

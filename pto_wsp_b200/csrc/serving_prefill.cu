@@ -693,6 +693,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 x[i] = *reinterpret_cast<const uint4*>(from + i * RPL * D);
                 if ((row & 15) >= live[side * 8 + (row >> 4)]) x[i] = make_uint4(0, 0, 0, 0);  // stale codes could be NaN
             }
+            // The reads are done, not only issued, before the next copy may write here: an arrival overtakes loads that
+            // queue behind a row's scattered stores.
+            fence_proxy_async_smem();
             arrive_warp(l_empty + 8 * side);
             if (s >= 2) ok = wait_for(empty + 8 * (s & 1), ((s >> 1) & 1) ^ 1u, abort_flag, a.status);
             if (!__all_sync(~0u, ok)) return;
