@@ -444,6 +444,21 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         const uint32_t meet_bar = meet_full + 8 * (x * 4 + (warp & 3));
         uint32_t tiles = 0, steps = 0, segments = 0, meets = 0;  // of this tile; of the CTA; of this tile; of these warps
         bool ok = true;
+        // Rows of q and of the output go between memory and this tile's place in shared memory with kRowLanes lanes side by
+        // side in a row; two warps share 32 rows, 16 each.  These loops and the converters' are rolled up on purpose: the
+        // roles' code has to stay in the instruction cache together.  For chunks of 1100-1500 rows over 2800-6200 keys
+        // (21864 steps) both rolled take 553 us; the converters unrolled over K and V 610, these loops unrolled as well 700.
+        // The softmax's inner loops lose when rolled up (568), and so does the MMA thread's over the two tiles (590).
+        constexpr int kRowLanes = D / 8, kRowsRead = 32 / kRowLanes;
+        const auto io_lane = []() {  // read anew at either use: what follows from it would hold registers across the steps
+            int i;
+            asm volatile("mov.u32 %0, %%laneid;" : "=r"(i));
+            return i;
+        };
+        const auto io_at = [&](int r, int unit) {
+            return reinterpret_cast<uint4*>(smem + S::kQ + x * S::kTile + (unit >> 3) * S::kBox + r * 128 +
+                                            (((unit & 7) ^ (r & 7)) << 4));
+        };
         // waits for the row's other thread; both warps come here alike
         const auto meet = [&]() {
             arrive_warp(meet_bar);
@@ -458,54 +473,67 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             }
             const int flat = w.p.row0 + x * 128 + row;
             const bool real = x * 128 + row < w.p.rows;
-            const int64_t tok = w.p.token0 + flat / a.group;
-            const int hq = w.head0 * a.group + flat % a.group;
             const int pos = real ? w.p.base + flat / a.group : -1;
-            // -- q as f16 times a power of two that brings the row's largest below 2^15 --
-            float factor;
+            // -- q as f16 times a power of two that brings the row's largest below 2^15: this warp's 16 rows --
             {
-                uint4 raw[D / 16];
-                const uint16_t* src = static_cast<const uint16_t*>(a.q) + tok * a.q_token_stride + hq * a.q_head_stride +
-                                      half * (D / 2);
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                    raw[i] = real ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
-                const bool f16 = a.dtype == PTOWSP_F16;
-                const auto value = [&](uint32_t u, int k) -> float {
-                    if (f16) return __half2float(__ushort_as_half(static_cast<unsigned short>(k ? u >> 16 : u & 0xffffu)));
-                    return __uint_as_float(k ? u & 0xffff0000u : u << 16);
-                };
-                float m = 0.f;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) m = fmaxf(m, fmaxf(fabsf(value(u[k], 0)), fabsf(value(u[k], 1))));
+                const int io = io_lane(), io_unit = io % kRowLanes, io_row = (warp & 3) * 32 + half * 16 + io / kRowLanes;
+                const int f0 = w.p.row0 + x * 128 + io_row;
+                int j = f0 / a.group, gq = f0 - j * a.group;
+#pragma unroll 1
+                for (int i = 0; i < 16; i += kRowsRead) {
+                    const bool there = x * 128 + io_row + i < w.p.rows;
+                    const uint16_t* src = static_cast<const uint16_t*>(a.q);
+                    if (there)
+                        src += (w.p.token0 + static_cast<int64_t>(j)) * a.q_token_stride +
+                               static_cast<int64_t>(w.head0 * a.group + gq) * a.q_head_stride + io_unit * 8;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(io_at(io_row + i, io_unit))),
+                                 "l"(src), "r"(there ? 16 : 0)
+                                 : "memory");
+                    for (gq += kRowsRead; gq >= a.group; gq -= a.group) ++j;
                 }
-                *mine = m;
-                meet();
-                if (!ok) break;
-                m = fmaxf(m, *other);
-                int e = 0;
-                if (m > 0.f && m < INFINITY)
-                    e = min(max(14 - (static_cast<int>(__float_as_uint(m) >> 23) - 127), -120), 120);
-                float f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-                factor = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                // The factor of the scores is positive, so a group's maximum is theirs and a masked score of -inf stays
-                // one: q takes the sign of the scale, or is zero with it.
-                if (a.scale < 0.f) f = -f;
-                if (a.scale == 0.f) f = 0.f;
+                asm volatile("cp.async.wait_all;" ::: "memory");  // a lane works on what it copied itself
+                const bool f16 = a.dtype == PTOWSP_F16;
+                float* factors = reinterpret_cast<float*>(smem + S::kMeet) + x * 2 * 128;
+#pragma unroll 1
+                for (int i = 0; i < 16; i += kRowsRead) {
+                    uint4* at = io_at(io_row + i, io_unit);
+                    const uint4 raw = *at;
+                    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+                    float v[8];
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-                    uint32_t h[4];
+                    for (int k = 0; k < 4; ++k) {
+                        if (f16) {
+                            const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
+                            v[2 * k] = t.x;
+                            v[2 * k + 1] = t.y;
+                        } else {
+                            v[2 * k] = __uint_as_float(u[k] << 16);
+                            v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+                        }
+                    }
+                    float m = 0.f;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) h[k] = pack2(value(u[k], 0) * f, value(u[k], 1) * f);
-                    const int unit = half * (D / 16) + i;
-                    *reinterpret_cast<uint4*>(smem + S::kQ + x * S::kTile + (unit >> 3) * S::kBox + row * 128 +
-                                              (((unit & 7) ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(v[k]));
+#pragma unroll
+                    for (int d = 1; d < kRowLanes; d <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+                    int e = 0;
+                    if (m > 0.f && m < INFINITY)
+                        e = min(max(14 - (static_cast<int>(__float_as_uint(m) >> 23) - 127), -120), 120);
+                    float f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                    if (io_unit == 0)
+                        factors[io_row + i] =
+                            fabsf(a.scale) * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                    // The factor of the scores is positive, so a group's maximum is theirs and a masked score of -inf
+                    // stays one: q takes the sign of the scale, or is zero with it.
+                    if (a.scale < 0.f) f = -f;
+                    if (a.scale == 0.f) f = 0.f;
+                    *at = make_uint4(pack2(v[0] * f, v[1] * f), pack2(v[2] * f, v[3] * f), pack2(v[4] * f, v[5] * f),
+                                     pack2(v[6] * f, v[7] * f));
                 }
             }
+            meet();
+            if (!ok) break;
+            const float factor = reinterpret_cast<const float*>(smem + S::kMeet)[x * 2 * 128 + row];
             fence_proxy_async_smem();
             arrive_warp(q_full + 8 * x);
 
@@ -542,23 +570,24 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 // the largest exponent
                 float top = -INFINITY;
                 {
-                    uint32_t r[2][32];
-                    tmem_ld32_async(s_cols, r[0]);
-                    tmem_ld32_async(s_cols + 32, r[1]);
-                    tmem_wait_ld();
-                    reg_fence(r[0]);
-                    reg_fence(r[1]);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const uint32_t* v = &r[q >> 1][(q & 1) * 16];
-                        float m0 = __uint_as_float(v[0]), m1 = __uint_as_float(v[1]);
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t r[32];
+                        tmem_ld32_async(s_cols + h * 32, r);
+                        tmem_wait_ld();
+                        reg_fence(r);
 #pragma unroll
-                        for (int c = 2; c < 16; c += 4) {
-                            m0 = fmaxf(fmaxf(m0, __uint_as_float(v[c])), __uint_as_float(v[c + 1]));
-                            if (c + 2 < 16) m1 = fmaxf(fmaxf(m1, __uint_as_float(v[c + 2])), __uint_as_float(v[c + 3]));
+                        for (int q = 0; q < 2; ++q) {
+                            const uint32_t* v = &r[q * 16];
+                            float m0 = __uint_as_float(v[0]), m1 = __uint_as_float(v[1]);
+#pragma unroll
+                            for (int c = 2; c < 16; c += 4) {
+                                m0 = fmaxf(fmaxf(m0, __uint_as_float(v[c])), __uint_as_float(v[c + 1]));
+                                if (c + 2 < 16) m1 = fmaxf(fmaxf(m1, __uint_as_float(v[c + 2])), __uint_as_float(v[c + 3]));
+                            }
+                            // a group without a page has a log2 of -inf
+                            top = fmaxf(top, fmaf(fmaxf(m0, m1), fmaxf(factor * sc[h * 2 + q], kLeast), sc[8 + h * 2 + q]));
                         }
-                        // a group without a page has a log2 of -inf
-                        top = fmaxf(top, fmaf(fmaxf(m0, m1), fmaxf(factor * sc[q], kLeast), sc[8 + q]));
                     }
                 }
                 // What a thread posts here its partner has read before the next time: the next scores wait for PV, and
@@ -628,23 +657,20 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             const bool any = l > 0.f || l != l;  // NaN goes through; a row that saw no key is zero
             const float inv = any ? 1.f / l : 0.f;
             float* part = g.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (w.unit0 > 0 ? 0 : 1)) * kRows * (D + 2);
+            // Every MMA of this tile is done: O takes the place of Q on its way out, whole as 16 bits, in parts as f32 in
+            // two passes.
 #pragma unroll 1
-            for (int c = 0; c < D / 64; ++c) {
-                uint32_t r[32];
-                tmem_ld32_async(o_cols + c * 32, r);
-                tmem_wait_ld();
-                reg_fence(r);
-                if (!real) continue;
-                const int dim = half * (D / 2) + c * 32;
-                if (w.whole) {
-                    uint16_t* to = static_cast<uint16_t*>(a.out) + tok * a.out_token_stride + hq * a.out_head_stride + dim;
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll 1
+                for (int d = 0; d < D / 4; d += 16) {
+                    uint32_t r[16];
+                    tmem_ld16(o_cols + c * (D / 4) + d, r);
+                    if (w.whole) {
+                        uint32_t h[8];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t h[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float v0 = any ? __uint_as_float(r[i * 8 + 2 * k]) * inv : 0.f;
-                            const float v1 = any ? __uint_as_float(r[i * 8 + 2 * k + 1]) * inv : 0.f;
+                        for (int k = 0; k < 8; ++k) {
+                            const float v0 = any ? __uint_as_float(r[2 * k]) * inv : 0.f;
+                            const float v1 = any ? __uint_as_float(r[2 * k + 1]) * inv : 0.f;
                             if (a.dtype == PTOWSP_F16) {
                                 h[k] = pack2(v0, v1);
                             } else {
@@ -652,22 +678,49 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                                 h[k] = *reinterpret_cast<const uint32_t*>(&b);
                             }
                         }
-                        *reinterpret_cast<uint4*>(to + i * 8) = make_uint4(h[0], h[1], h[2], h[3]);
-                    }
-                } else {
-                    float* to = part + 2 * kRows + (x * 128 + row) * D + dim;
+                        const int unit = half * (D / 16) + c * (D / 32) + d / 8;
+                        *io_at(row, unit) = make_uint4(h[0], h[1], h[2], h[3]);
+                        *io_at(row, unit + 1) = make_uint4(h[4], h[5], h[6], h[7]);
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        *reinterpret_cast<uint4*>(to + i * 4) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+                        for (int i = 0; i < 4; ++i)
+                            *io_at(row, half * (D / 16) + d / 4 + i) =
+                                make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+                    }
+                }
+                if (w.whole && c == 0) continue;
+                meet();
+                if (!ok) break;
+                const int io = io_lane(), io_unit = io % kRowLanes, io_row = (warp & 3) * 32 + half * 16 + io / kRowLanes;
+                const int f0 = w.p.row0 + x * 128 + io_row;
+                int j = f0 / a.group, gq = f0 - j * a.group;
+#pragma unroll 1
+                for (int r = io_row; r < (warp & 3) * 32 + half * 16 + 16 && x * 128 + r < w.p.rows; r += kRowsRead) {
+                    const uint4 v = *io_at(r, io_unit);
+                    if (w.whole) {
+                        *reinterpret_cast<uint4*>(
+                            static_cast<uint16_t*>(a.out) + (w.p.token0 + static_cast<int64_t>(j)) * a.out_token_stride +
+                            static_cast<int64_t>(w.head0 * a.group + gq) * a.out_head_stride + io_unit * 8) = v;
+                        for (gq += kRowsRead; gq >= a.group; gq -= a.group) ++j;
+                    } else {
+                        const int dim = io_unit / (D / 16) * (D / 2) + c * (D / 4) + io_unit % (D / 16) * 4;
+                        *reinterpret_cast<uint4*>(part + 2 * kRows + (x * 128 + r) * D + dim) = v;
+                    }
+                }
+                if (!w.whole && c == 0) {
+                    meet();  // both have read what the second pass writes over
+                    if (!ok) break;
                 }
             }
+            if (!ok) break;
             tc_fence_before();  // O has been read: the next segment's first PV comes after this thread's next P
             if (real && half == 0) {
                 if (!w.whole) {
                     part[(x * 128 + row) * 2] = M;
                     part[(x * 128 + row) * 2 + 1] = l;
                 } else if (a.lse) {
-                    a.lse[tok * a.heads + hq] = any ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
+                    const int j = flat / a.group;
+                    a.lse[(w.p.token0 + static_cast<int64_t>(j)) * a.heads + w.head0 * a.group + flat - j * a.group] = any ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
                 }
             }
         }
@@ -693,8 +746,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 x[i] = *reinterpret_cast<const uint4*>(from + i * RPL * D);
                 if ((row & 15) >= live[side * 8 + (row >> 4)]) x[i] = make_uint4(0, 0, 0, 0);  // stale codes could be NaN
             }
-            // The reads are done, not only issued, before the next copy may write here: an arrival overtakes loads that
-            // queue behind a row's scattered stores.
+            // The reads are done, not only issued, before the next copy may write here: an arrival can overtake loads
+            // that stand in a queue.
             fence_proxy_async_smem();
             arrive_warp(l_empty + 8 * side);
             if (s >= 2) ok = wait_for(empty + 8 * (s & 1), ((s >> 1) & 1) ^ 1u, abort_flag, a.status);
@@ -719,8 +772,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             arrive_warp(full + 8 * (s & 1));
         };
         for (int s = 0; s < steps && __all_sync(~0u, ok); ++s) {
-            convert(0, s, k_full, k_empty, smem + S::kK);
-            if (__all_sync(~0u, ok)) convert(1, s, v_full, v_empty, smem + S::kV);
+#pragma unroll 1
+            for (int side = 0; side < 2 && __all_sync(~0u, ok); ++side)  // one copy of the code
+                convert(side, s, k_full + 32 * side, k_empty + 32 * side, smem + S::kK + side * (S::kV - S::kK));
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
