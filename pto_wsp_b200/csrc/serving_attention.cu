@@ -10,6 +10,11 @@
 // Codes become f16 exactly (e4m3 and int8 are subsets of it).  A row of q enters as f16 times a power of two that
 // brings its largest element below 2^15, which is exact for f16 and for bf16 elements down to 2^-29 of the row's
 // largest; below that the lost part is under 2^-39 of it.  Sums are f32 in the MMA and in registers.
+//
+// Bound by HBM: every code is read once.  64 requests of one token over 512-8192 keys (8 KV heads of 128, groups of four:
+// 582 MB) take 108 us as a whole call, 5.4 TB/s; the copy rate would take 89.  Three requests over 100,000-200,000 keys:
+// 114 us for 599 MB.  What is left is the second launch and the CTAs' ends, some 8 us, and the warps' waits for boxes of
+// 2 to 4 KB, which 16 bytes per thread by cp.async (118 us) and plain loads (128) served worse.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -811,8 +816,9 @@ cudaError_t launch_d(const AttendArgs& a, int sms, cudaStream_t s) {
     }
 }
 
-// Above so many q rows of a request the tcgen05 kernel is faster although it pads them to 128: a tile of 32 rows takes
-// the warp MMAs about 1.4 times as long as its codes take from HBM, and every further tile as long again.
+// Above so many q rows of a request and KV head the tcgen05 kernel is faster although it pads them to 128: the warp MMAs
+// read the codes once per 32 rows.  32 requests of 8 KV heads over 4096 keys each: 32 rows take 122 us here and 173
+// there, 40 rows 208 here and 175 there.
 constexpr int kFew = 32;
 
 size_t few_bytes(const AttendArgs& a, int sms) {

@@ -16,6 +16,9 @@ namespace {
 // from three prefix sums over the requests (tokens, needed pages, returned pages).  Every CTA runs the sums for
 // itself -- a thousand requests are one round of a block scan, cheaper than a second launch -- keeps the two that the
 // token list needs in shared memory and then fills its share of the outputs; CTA 0 writes the per-request ones.
+//
+// Bound by latency: 6 us on the device for 64 requests of one token, 12 for 1001 requests with 0-511 each, of a whole call
+// of 18 us in which the host allocates six results.
 // ---------------------------------------------------------------------------
 
 constexpr int kRsvThreads = 1024;
@@ -166,7 +169,9 @@ __global__ void __launch_bounds__(kRsvThreads) reserve_kernel(ReserveArgs a) {
 // run, which the CTA that holds its first token writes to its end (at most a page).  Many short runs (decoding): a warp
 // each; few long ones (prefill): the warps share each, so that its rows are all under way at once and are read once.
 //
-// Bound by HBM: 2 or 4 bytes in and 1 out per element.
+// Bound by HBM in principle, 2 or 4 bytes in and 1 out per element; in fact by instructions and the runs' fixed parts:
+// 16,001 tokens of 8 heads of 128 in f16 to int8 (98 MB) take 46 us, 2.1 TB/s, of which rounding is a sixth.  One warp
+// per run took 128 us there.  64 single tokens take 8.5 us, 4.4 of them on the device.
 // ---------------------------------------------------------------------------
 
 constexpr int kAppWarps = 8;

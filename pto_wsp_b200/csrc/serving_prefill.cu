@@ -17,8 +17,13 @@
 //   warp 20         issues the MMAs from one thread: S_A S_B | PV_A S_A' | PV_B S_B' | ...: while the tensor cores work
 //                   on one tile's products the other tile's softmax runs
 //   warp 21         asks for the codes by TMA, a box per 16 tokens, and gives the groups' scales
-// TMEM: S_A, S_B (128 columns each; P over the first 32 of either half), O_A, O_B.  The tensor pipe runs one thread's MMAs in order, so
-// S' may follow PV into the columns that P is read from, and S' being done means that PV is.
+// TMEM: S_A, S_B (128 columns each; P over the first 32 of either half), O_A, O_B.  The tensor pipe runs one thread's MMAs
+// in order, so S' may follow PV into the columns that P is read from, and S' being done means that PV is.
+//
+// Bound by the tensor pipe's feed and by the chain score - softmax - product of a tile.  Chunks of 1142-1516 rows over
+// 2791-6204 keys (8 KV heads, groups of four, D = 128: 355 GFLOP) take 553 us, 643 TFLOP/s; both products of a step take
+// 2048 cycles at the full rate and some 3000 here, seen from the issuing thread: Q and K tiles, the conversion and the
+// copies share shared memory's 128 bytes a cycle.  The rest is the chain's, and a CTA's way from one task to the next.
 //
 // Work is dealt out as for few rows: the steps of all (tile pair, head) tasks stand in one line, every CTA takes an equal
 // part, and tasks that this cuts are joined by a second launch.  A first launch lists the tile pairs.

@@ -6,9 +6,16 @@
 // need no counting.
 //
 // A cluster of CTAs holds a row in shared memory: it is read from HBM once, and every pass after that -- maximum,
-// counts, masses, the pick -- runs over the copy.  A cut is found by a histogram over the logits' distance from the
-// maximum (evenly spaced, where a radix over the bits would put most of a row into a few bins), and the elements of the
-// bin that holds it are ranked against one another; a bin with too many is divided again over its range of composites.
+// counts, masses, the pick -- runs over the copy.  The logits' distance from the maximum is cut into even bins, where a
+// radix over the bits would put most of a row into a few.  Top-k lists the likely elements and ranks them against one
+// another.  Top-p counts the elements of each bin; a bin's edges bound its mass, so counts alone leave a window of few
+// bins that can hold the cut, and only the window is summed by mass.  A bin with too many elements is divided again
+// over its range of composites.
+//
+// Bound by a row's chain of barriers: a pass over a slice in shared memory takes about a microsecond, and each pass waits
+// for the one before.  One row of 50,021 (top-p) takes 26 us, 64 rows of 131,072 with all filters 29 us (17 MB, 0.6
+// TB/s), 509 rows of 32,000 without filters 37.6 us (65 MB, 1.7 TB/s).  Two rows in flight per cluster took 60 for the
+// last, slices read from L1 and L2 instead of shared memory 37-52.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
