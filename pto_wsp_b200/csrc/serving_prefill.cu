@@ -335,7 +335,7 @@ struct Smem {
     static constexpr int kLive = kScales + 4 * 3 * 8 * 4;  // [2][8]: tokens of a landed group that are there
     static constexpr int kMeet = kLive + 2 * 8 * 4;      // [2 tiles][2 halves][128]: what a row's threads tell each other
     static constexpr int kBars = kMeet + 2 * 2 * 128 * 4;
-    static constexpr int kBytes = kBars + 320;           // dynamic shared memory begins at a multiple of 1024
+    static constexpr int kBytes = kBars + 256;           // dynamic shared memory begins at a multiple of 1024
 };
 static_assert(Smem<128>::kBytes <= 232448, "227 KB of shared memory per CTA");
 
@@ -377,13 +377,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
     const uint32_t bar0 = smem_u32(bars);
     const uint32_t q_full = bar0, k_full = bar0 + 16, k_empty = bar0 + 32, v_full = bar0 + 48, v_empty = bar0 + 64,
-                   sc_full = bar0 + 80, s_full = bar0 + 112, p_full = bar0 + 128, o_full = bar0 + 144, drain = bar0 + 160,
-                   l_full = bar0 + 168, l_empty = bar0 + 184;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 25);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+                   s_full = bar0 + 80, p_full = bar0 + 96, o_full = bar0 + 112, drain = bar0 + 128, l_full = bar0 + 136,
+                   l_empty = bar0 + 152;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 21);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
     volatile int* live = reinterpret_cast<volatile int*>(smem + S::kLive);
-    volatile int* first_pair = reinterpret_cast<volatile int*>(bars + 27);
-    const uint32_t meet_full = bar0 + 224;  // [2][4]: of a tile, by the row's quarter
+    volatile int* first_pair = reinterpret_cast<volatile int*>(bars + 23);
+    const uint32_t meet_full = bar0 + 192;  // [2][4]: of a tile, by the row's quarter
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     const int64_t total = g.total[0];
@@ -408,7 +408,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             mbar_init(l_full + 8 * i, 1);
             mbar_init(l_empty + 8 * i, 4);
         }
-        for (int i = 0; i < 4; ++i) mbar_init(sc_full + 8 * i, 1);
         for (int i = 0; i < 8; ++i) mbar_init(meet_full + 8 * i, 2);
         mbar_init(drain, 1);
         *abort_flag = 0;
@@ -551,9 +550,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             for (int j = 0; j < w.n; ++j, key0 += kKeys) {
                 const bool plain = key0 + kKeys <= min(low + 1, w.p.hi) && (a.window == 0 || key0 > high - a.window);
                 const float* sc = scales + (steps & 3) * 24 + half * 4;
-                ok = wait_for(sc_full + 8 * (steps & 3), (steps >> 2) & 1, abort_flag, a.status) &&
-                     wait_for(s_full + 8 * x, tiles & 1, abort_flag, a.status);
-                ok = __all_sync(~0u, ok);  // the TMEM loads are the whole warp's
+                // The scores being there, the step's scales are.  The TMEM loads are the whole warp's.
+                ok = __all_sync(~0u, wait_for(s_full + 8 * x, tiles & 1, abort_flag, a.status));
                 if (!ok) break;
                 tc_fence_after();
                 ++steps;
@@ -822,6 +820,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 if (s > 0) ok = __all_sync(~0u, wait_for(l_empty + 8 * side, (s - 1) & 1, abort_flag, a.status));
                 if (!ok) break;
                 if (lane < 8) live[side * 8 + lane] = count;
+                if (side == 0 && lane < 8) {
+                    // The scales go before K's arrival: whoever has this step's scores has its scales by the chain
+                    // landed - converted - multiplied.  (A barrier of their own would not do: a tile that sits out short
+                    // pairs comes to it any number of phases early, where the parity of an old phase lets it pass.)
+                    // Slot s & 3 was last read in step s - 4: K of step s - 1 has been read, so V of step s - 2 has been
+                    // converted, for which PV of step s - 4 had to be done, and with it both tiles' softmax.
+                    float* to = scales + (s & 3) * 24 + lane;
+                    const bool any = here >= 0 && ks > 0.f;  // a group without a page: log2 -inf, nothing to the sum
+                    to[0] = any ? ks : 0.f;
+                    to[8] = any ? log2f(vs) : -INFINITY;
+                    to[16] = any ? 1.f / vs : 0.f;
+                }
                 __syncwarp();
                 if (lane == 0) mbar_expect_tx(l_full + 8 * side, __popc(there) * 16 * D);
                 __syncwarp();
@@ -829,19 +839,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     tma_load_page(sQ - S::kQ + S::kLand + side * kKeys * D + lane * 16 * D, side ? &v_map : &k_map, h, tok,
                                   here, l_full + 8 * side);
                 asked = 2 * s + side + 1;
-                if (side == 0) {
-                    // slot s & 3 was last read in step s - 4: V of step s - 2 has been converted, for which PV of step
-                    // s - 4 had to be done, and with it both tiles' softmax
-                    const int slot = s & 3;
-                    if (lane < 8) {  // a group without a page: log2 -inf, nothing to the sum
-                        const bool any = here >= 0 && ks > 0.f;
-                        scales[slot * 24 + lane] = any ? ks : 0.f;
-                        scales[slot * 24 + 8 + lane] = any ? log2f(vs) : -INFINITY;
-                        scales[slot * 24 + 16 + lane] = any ? 1.f / vs : 0.f;
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(sc_full + 8 * slot);
-                    // the next step's page and scales
+                if (side == 0) {  // the next step's page and scales
                     ++at;
                     if (++unit == p.units && at < w.stop) {
                         unit = 0;

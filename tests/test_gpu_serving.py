@@ -525,6 +525,23 @@ def test_attend_gives_the_same_bits_every_time(fmt, group, qs):
     assert all(torch.equal(o, first) and torch.equal(l, first_lse) for o, l in runs)
 
 
+@pytest.mark.parametrize("fmt,heads,group,dim", [("e4m3", 2, 2, 128), ("int8", 1, 4, 64)])
+def test_attend_full_tiles_after_short_ones(fmt, heads, group, dim):
+    # 256 and then 24 to 104 rows per request and head: one of the two row tiles sits the second part out, whose number of
+    # steps varies, and comes back where the pages' scales are others, up to 2^15 apart.
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    qs = [(256 + 24 + 16 * (i % 6)) // group for i in range(150)]
+    lens = [m + 37 * (i % 23) for i, m in enumerate(qs)]
+    (k, ks), (v, vs) = (made := paged(fmt, lens, 16, heads, dim, "hnd", gen, spread=2.0))[0]
+    q = (0.5 * torch.randn(sum(qs), heads * group, dim, generator=gen, device="cuda")).half()
+    args = (q, k, v, ks, vs, made[1], dev(lens, torch.int32))
+    more = {"q_start": dev(np.cumsum([0] + qs), torch.int32), "max_q": max(qs), "return_lse": True}
+    first, first_lse = serving.attend_kv8(*args, **more)
+    check_attention(first, first_lse, attention_reference(q, made[2], lens, qs, 0, dim ** -0.5), q.dtype)
+    runs = [serving.attend_kv8(*args, **more) for _ in range(50)]
+    assert all(torch.equal(o, first) and torch.equal(l, first_lse) for o, l in runs)
+
+
 def test_attend_offsets_beyond_32_bits():
     pages, page, heads, dim = 140_000, 16, 8, 128  # 2.3e9 codes
     gen = torch.Generator(device="cuda").manual_seed(6)
