@@ -255,7 +255,7 @@ enum ptowsp_serving_status {
     PTOWSP_SERVING_PAGE = 1,    /* a page id or slot outside the cache */
     PTOWSP_SERVING_LENGTH = 2,  /* a length that is negative, or beyond the page table */
     PTOWSP_SERVING_REFUSED = 4, /* a request's new tokens found no room (pages, table or token list) */
-    PTOWSP_SERVING_RING = 8,    /* the free-page ring's state is inconsistent (too many pages given back) */
+    PTOWSP_SERVING_RING = 8,    /* the free-page ring's state is inconsistent, or too many pages are given back */
     PTOWSP_SERVING_TIMEOUT = 16 /* a bounded wait inside a kernel gave up: the output is not complete */
 };
 
@@ -264,7 +264,8 @@ enum ptowsp_serving_status {
  *   kv_len      i32 [requests]  tokens each request has in the cache
  *   new_tokens  i32 [requests]  tokens to come; negative: the request ended
  *   free_ring   i32 [ring_size] free page ids at places head .. tail - 1, modulo ring_size
- *   free_state  i64 [2]         (head, tail), 0 <= tail - head <= ring_size
+ *   free_state  i64 [2]         (head, tail), 0 <= head, 0 <= tail - head <= ring_size; any other state is reported, gives
+ *                               no page and takes none back
  * Requests are served in order; one whose pages the ring does not have, or whose tokens pass the table or
  * `max_tokens`, is refused (its length stays, its slots are -1).  Pages of ended requests go behind the tail and are
  * given out from the next call on.  Results, none aliasing an input:

@@ -60,7 +60,9 @@ __global__ void __launch_bounds__(kRsvThreads) reserve_kernel(ReserveArgs a) {
     const int64_t head = a.free_state[0], tail = a.free_state[1];
     int64_t avail = tail - head;
     int flags = 0;
-    if (avail < 0 || avail > a.ring_size || head < 0) {
+    // such a ring gives no page and takes none; the last comparison keeps the places behind the tail countable
+    const bool broken = head < 0 || tail < head || avail > a.ring_size || tail > INT64_MAX - a.ring_size;
+    if (broken) {
         avail = 0;
         flags |= PTOWSP_SERVING_RING;
     }
@@ -112,7 +114,7 @@ __global__ void __launch_bounds__(kRsvThreads) reserve_kernel(ReserveArgs a) {
             if (t.back) taken[r] = -2 - static_cast<int32_t>(be - t.back < INT32_MAX - 2 ? be - t.back : INT32_MAX - 2);
         }
     }
-    const bool overflow = avail + back_before > a.ring_size;  // more pages than the ring has places
+    const bool overflow = broken || avail + back_before > a.ring_size;  // more pages than the ring has places
     if (overflow) flags |= PTOWSP_SERVING_RING;
     if (first && threadIdx.x == 0) {
         a.q_start[0] = 0;

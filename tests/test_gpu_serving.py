@@ -148,6 +148,21 @@ def test_reserve_reports_a_broken_ring_and_bad_lengths():
     serving.check_status(status)
 
 
+@pytest.mark.parametrize("state", [[0, -3], [-5, -3], [-2, 1], [5, 2], [0, 9], [-(2 ** 63), 0], [0, 2 ** 63 - 1],
+                                   [2 ** 63 - 3, 2 ** 63 - 2]])
+def test_reserve_leaves_a_broken_ring_alone(state):
+    wide = torch.arange(100, 112, dtype=torch.int32, device="cuda")
+    ring, before = wide[4:8], wide.clone()  # words on both sides that nothing may touch
+    table = torch.tensor([[50, 51, 0, 0], [60, 0, 0, 0], [70, 0, 0, 0]], dtype=torch.int32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    step = serving.reserve_pages(table.clone(), dev([20, 16, 3], torch.int32), dev([-1, 1, 1], torch.int32), ring,
+                                 torch.tensor(state, device="cuda"), page_size=16, max_tokens=8, status=status)
+    assert int(status) == serving.RING | serving.REFUSED  # no page for request 1; request 2 has room in its own
+    assert torch.equal(wide, before) and step.free_state.tolist() == state
+    assert step.granted.tolist() == [False, False, True] and step.kv_len.tolist() == [0, 16, 4]
+    assert step.slots.tolist() == [-1, 70 * 16 + 3] + [-1] * 6
+
+
 def test_reserve_without_requests():
     e = torch.empty(0, dtype=torch.int32, device="cuda")
     step = serving.reserve_pages(e.reshape(0, 4), e, e, torch.arange(3, dtype=torch.int32, device="cuda"),
