@@ -336,11 +336,11 @@ PTOWSP_API int ptowsp_cuda_kv8_append(const ptowsp_kv8_cache* cache, const ptows
  *   lse         f32 [tokens][num_heads], or NULL: log of the sum of the exponentials
  *   page_table  i32 [requests][max_pages], rows `table_stride` apart
  *   kv_len      i32 [requests], the new tokens included
- *   q_start     i32 [requests + 1], q rows of request r: q_start[r] .. q_start[r + 1] - 1; NULL: row r
- *   max_q       the most rows that any request has
+ *   q_start     i32 [requests + 1], not falling, q rows of request r: q_start[r] .. q_start[r + 1] - 1; NULL: row r
+ *   max_q       the most rows that any request has; one with more is left out and reported
  *   window      > 0: a row sees its own token and the window - 1 before it; 0: all before it
- * Row j of nq sees the keys t <= kv_len - nq + j.  A row that sees none gets zeros and lse = -inf.  A page id
- * outside the cache hides its tokens.  `workspace`: ptowsp_cuda_kv8_attention_workspace bytes, 256-byte aligned,
+ * Row j of nq sees the keys t <= kv_len - nq + j.  A row that sees none gets zeros and lse = -inf, and so does one that
+ * no request has or whose request is left out.  A page id outside the cache hides its tokens.  `workspace`: ptowsp_cuda_kv8_attention_workspace bytes, 256-byte aligned,
  * contents irrelevant, used until the call's work on the stream is done. */
 typedef struct ptowsp_kv8_attention_args {
     const void* q;

@@ -190,8 +190,8 @@ int ptowsp_cuda_kv8_attention(const ptowsp_kv8_cache* cache, const ptowsp_kv8_at
     AttendArgs a{};
     int rc = attend_of(cache, g, &a);
     if (rc != PTOWSP_OK) return rc;
-    if (a.requests == 0 || a.tokens == 0) return PTOWSP_OK;
-    if (!a.q || !a.out || !a.kv_len || (a.max_pages && !a.page_table))
+    if (a.tokens == 0) return PTOWSP_OK;
+    if (!a.q || !a.out || (a.requests && (!a.kv_len || (a.max_pages && !a.page_table))))
         return fail(PTOWSP_ERR_ARG, "%s: null pointer", what);
     if (!a.q_start && (a.tokens != a.requests || a.max_q != 1))
         return fail(PTOWSP_ERR_ARG, "%s: without q_start every request has one token (max_q 1)", what);

@@ -142,6 +142,8 @@ struct Deal {
     int64_t ctas;         // CTAs that share them
     int64_t share, rest;  // steps of each, and the first CTAs that have one more
     int per;              // requests per thread of the scan
+    bool left_out;        // a request may have been left out
+    bool loose;           // that, or rows before the first request's or behind the last one's
 
     __device__ __forceinline__ int64_t start(int64_t c) const { return c * share + (c < rest ? c : rest); }
     // the CTA that has step i
@@ -155,6 +157,7 @@ template <int ROWS>
 __device__ Deal deal_out(const AttendArgs& a, int ctas, int64_t* sums, int* flags) {
     Deal d;
     d.per = (a.requests + kThreads - 1) / kThreads;
+    const bool ends = a.q_start && threadIdx.x == 0 && (a.q_start[0] != 0 || a.q_start[a.requests] < a.tokens);
     int64_t mine = 0;
     for (int i = 0; i < d.per; ++i) {
         const int r = threadIdx.x * d.per + i;
@@ -174,7 +177,8 @@ __device__ Deal deal_out(const AttendArgs& a, int ctas, int64_t* sums, int* flag
     __syncthreads();
     for (int w = 0; w < warp; ++w) v += warp_sum[w];
     sums[threadIdx.x] = v;  // inclusive
-    __syncthreads();
+    d.loose = __syncthreads_or(*flags || ends);
+    d.left_out = d.loose && __syncthreads_or(*flags);
     d.total = sums[kThreads - 1];
     d.ctas = d.total < ctas ? (d.total > 0 ? d.total : 1) : ctas;
     d.share = quotient(d.total, d.ctas);
@@ -239,6 +243,33 @@ __device__ __forceinline__ void store_row(const AttendArgs& a, int row0, int hea
     if (first && a.lse) a.lse[tok * a.heads + hq] = any ? (m + log2f(sum)) * 0.6931471805599453f : -INFINITY;
 }
 
+// Rows of q that no request has -- before the first one's or behind the last one's, as where the rows are padded to a
+// fixed number, and those of a request that was left out -- get zeros and lse = -inf.  `some`: a request may have been
+// left out, so every row is looked up; else only the ends are.  A warp per row.
+template <int D>
+__device__ __noinline__ void clear_rows(const AttendArgs& a, bool some) {
+    const int lane = threadIdx.x & 31;
+    const int begin = a.q_start[0], end = a.q_start[a.requests];
+    const int64_t skip = !some && begin == 0 ? end : 0;
+    for (int64_t t = skip + blockIdx.x * kWarps + (threadIdx.x >> 5); t < a.tokens; t += gridDim.x * kWarps) {
+        if (t >= begin && t < end) {
+            int lo = 0, hi = a.requests - 1;  // the request whose rows these are: the first that ends behind t
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (a.q_start[mid + 1] > t) hi = mid;
+                else lo = mid + 1;
+            }
+            const int row0 = a.q_start[lo], row1 = a.q_start[lo + 1];
+            if (row0 >= 0 && row1 <= a.tokens && row1 - row0 <= a.max_q) continue;
+        }
+        for (int h = 0; h < a.heads; ++h) {
+            char* to = static_cast<char*>(a.out) + (t * a.out_token_stride + h * a.out_head_stride) * 2;
+            if (lane < D / 8) reinterpret_cast<uint4*>(to)[lane] = make_uint4(0, 0, 0, 0);
+            if (lane == 0 && a.lse) a.lse[t * a.heads + h] = -INFINITY;
+        }
+    }
+}
+
 template <int D, int NB>
 struct Layout {
     static constexpr int ROWS = 8 * NB;
@@ -282,6 +313,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NB)) attend_kernel(const
     int flags = 0;
     const Deal deal = deal_out<ROWS>(a, gridDim.x, sums, &flags);
     if (blockIdx.x == 0 && flags && a.status) atomicOr(a.status, flags);
+    if (a.q_start && deal.loose) clear_rows<D>(a, deal.left_out);
     if (deal.total == 0 || blockIdx.x >= deal.ctas) {
         if (threadIdx.x == 0) cut->pieces = 0;
         return;
@@ -852,10 +884,10 @@ size_t attend_workspace_bytes(const AttendArgs& args, int sms) {
 }
 
 cudaError_t launch_attend(const AttendArgs& args, int sms, cudaStream_t s) {
-    if (args.requests == 0 || args.tokens == 0) return cudaSuccess;
+    if (args.tokens == 0) return cudaSuccess;
     const AttendArgs a = split(args);
     cudaError_t e = cudaSuccess;
-    if (a.few) e = launch_prefill(a, kFew, a.workspace + few_bytes(a, sms), sms, s);
+    if (a.few && a.requests > 0) e = launch_prefill(a, kFew, a.workspace + few_bytes(a, sms), sms, s);
     if (e != cudaSuccess) return e;
     if (a.cache.format == PTOWSP_KV8_E4M3)
         return a.cache.head_dim == 64 ? launch_d<PTOWSP_KV8_E4M3, 64>(a, sms, s) : launch_d<PTOWSP_KV8_E4M3, 128>(a, sms, s);

@@ -222,15 +222,17 @@ def append_kv8(k, v, slots, k_cache, v_cache, k_scale, v_scale, *, status=None) 
         tokens, dtype, 0, _vector(status, "status", torch.int32, 1, index)))
 
 
-def attend_kv8(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_len, *, q_start=None, max_q: int = 1, scale=None,
+def attend_kv8(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_len, *, q_start=None, max_q: int | None = None, scale=None,
                window: int = 0, out=None, return_lse: bool = False, status=None):
     """Causal attention of each request's newest tokens over its cached ones.
 
     ``q`` [tokens, heads, head_dim] in float16 or bfloat16, one row per request, or rows ``q_start[r]`` ..
-    ``q_start[r + 1] - 1`` (int32 [requests + 1]) of request r, at most ``max_q``.  ``kv_len`` int32 [requests] counts
+    ``q_start[r + 1] - 1`` (int32 [requests + 1]) of request r, at most ``max_q`` (unless given: all of them, which a
+    batch of short requests pays for with the launches for long ones).  ``kv_len`` int32 [requests] counts
     the cached tokens, the new ones included, whose pages stand in ``page_table`` int32 [requests, max_pages].
     ``scale`` of the scores: 1 / sqrt(head_dim) unless given; ``window`` > 0: a row sees its own token and the
-    window - 1 before it.  Returns out like q, and with ``return_lse`` also float32 [tokens, heads]."""
+    window - 1 before it.  Returns out like q, and with ``return_lse`` also float32 [tokens, heads].  Rows that see no
+    key, that no request has, or whose request has more than ``max_q`` (also reported) are zeros with an lse of -inf."""
     index, cache, _, dim = _cache(k_cache, v_cache, k_scale, v_scale)
     dtype = _DTYPES.get(q.dtype)
     if not dtype:
@@ -245,6 +247,8 @@ def attend_kv8(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_len, *, q_s
         os = out.stride()
         if out.shape != shape or out.dtype is not q.dtype or out.get_device() != index or os[2] != 1:
             raise ValueError("out must be like q")
+    if max_q is None:
+        max_q = 1 if q_start is None else tokens
     i32 = torch.int32
     requests = kv_len.shape[0]
     table, stride, max_pages = _table(page_table, requests, index)

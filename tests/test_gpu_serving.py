@@ -557,6 +557,59 @@ def test_attend_full_tiles_after_short_ones(fmt, heads, group, dim):
     assert all(torch.equal(o, first) and torch.equal(l, first_lse) for o, l in runs)
 
 
+@pytest.mark.parametrize("qs,max_q", [([1, 5, 2, 0, 3], 3), ([1, 40, 2, 70, 3], 64), ([2, 4, 1, 3, 1], 1)])
+@pytest.mark.parametrize("front,back", [(0, 0), (3, 0), (0, 50), (2, 700)])
+def test_attend_rows_without_a_request(qs, max_q, front, back):
+    # rows before the first request's and behind the last one's, and requests of more rows than max_q: zeros, lse -inf
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    lens = [100, 90, 33, 12, 400]
+    (k, ks), (v, vs) = (made := paged("e4m3", lens, 16, 2, 64, "hnd", gen))[0]
+    rows = front + sum(qs) + back
+    q = torch.randn(rows, 8, 64, generator=gen, device="cuda").half()
+    start = np.cumsum([front] + qs)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    wide = torch.full((rows, 8, 96), math.nan, dtype=q.dtype, device="cuda")
+    out = wide[:, :, 16:80]
+    del_me = torch.full((rows, 8), math.nan, device="cuda")  # where lse will probably stand
+    del del_me
+    _, lse = serving.attend_kv8(q, k, v, ks, vs, made[1], dev(lens, torch.int32), q_start=dev(start, torch.int32),
+                                max_q=max_q, return_lse=True, status=status, out=out)
+    want = attention_reference(q[front:front + sum(qs)], made[2], lens, qs, 0, 0.125)
+    taken = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    for a, m in zip(start, qs):
+        if m <= max_q:
+            taken[a:a + m] = True
+    inner = taken[front:front + sum(qs)]
+    check_attention(out[taken], lse[taken], [c[inner] for c in want], q.dtype)
+    assert not out[~taken].any() and bool((lse[~taken] == -math.inf).all())
+    assert bool(torch.isnan(wide[:, :, :16]).all()) and bool(torch.isnan(wide[:, :, 80:]).all())
+    assert int(status) == (serving.LENGTH if max(qs) > max_q else 0)
+
+
+@pytest.mark.parametrize("qs", [[1, 1, 1], [3, 1, 4], [60, 1, 40]])
+def test_attend_without_max_q(qs):
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    lens = [100, 90, 300]
+    (k, ks), (v, vs) = (made := paged("int8", lens, 16, 2, 128, "nhd", gen))[0]
+    q = torch.randn(sum(qs), 8, 128, generator=gen, device="cuda").bfloat16()
+    out, lse = serving.attend_kv8(q, k, v, ks, vs, made[1], dev(lens, torch.int32), return_lse=True,
+                                  q_start=dev(np.cumsum([0] + qs), torch.int32))
+    check_attention(out, lse, attention_reference(q, made[2], lens, qs, 0, 128 ** -0.5), q.dtype)
+
+
+def test_attend_rows_without_any_request():
+    gen = torch.Generator(device="cuda").manual_seed(10)
+    (k, ks), (v, vs) = (made := paged("int8", [20], 16, 2, 64, "nhd", gen))[0]
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    for rows in (1, 100):
+        q = torch.randn(rows, 4, 64, device="cuda").half()
+        out, lse = serving.attend_kv8(q, k, v, ks, vs, made[1][:0], none, q_start=dev([0], torch.int32), return_lse=True,
+                                      out=torch.full_like(q, math.nan))
+        assert not out.any() and bool((lse == -math.inf).all())
+        with pytest.raises(PtoWspCudaError):  # a row per request, but there is none
+            serving.attend_kv8(q, k, v, ks, vs, made[1][:0], none)
+
+
 def test_attend_offsets_beyond_32_bits():
     pages, page, heads, dim = 140_000, 16, 8, 128  # 2.3e9 codes
     gen = torch.Generator(device="cuda").manual_seed(6)
