@@ -496,8 +496,9 @@ cudaError_t append_t(const AppendArgs& a, dim3 grid, int chunk, cudaStream_t s) 
 
 cudaError_t launch_reserve(const ReserveArgs& a, cudaStream_t s) {
     const int smem = std::max(1, a.requests) * 8;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(reserve_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (smem > 47 * 1024) {  // with the kernel's static words more than 48 KB
+        static SmemOptIn opt_in;  // for the most requests at once: a limit of this call's size would be another thread's too
+        const cudaError_t e = opt_in.once(reinterpret_cast<const void*>(reserve_kernel), kReserveMaxRequests * 8);
         if (e != cudaSuccess) return e;
     }
     // one CTA per 4096 tokens or 256 requests: below that the extra CTAs' own prefix sums cost more than they save

@@ -126,6 +126,37 @@ def test_reserve_against_the_definition(requests, page, max_len, new, max_pages,
         status.zero_()
 
 
+@pytest.mark.parametrize("order", [[6016, 6017, 6112, 6144, 6145, 16384, 6145], [16384, 7000, 16384, 1]])
+def test_reserve_of_many_requests(order):
+    # more than some 6100 requests take more shared memory than a kernel has unasked; a smaller call may not lower the limit
+    rng = np.random.default_rng(1)
+    for requests in order:
+        table, lens, new, ring, free, page, total = reserve_case(rng, requests, 16, 40, lambda g, n: g.integers(-1, 4, n),
+                                                                 4, 9000, 5)
+        want = reserve_reference(table, lens.tolist(), new.tolist(), ring, free, page, total)
+        t, ring_d = dev(table, torch.int32), dev(ring, torch.int32)
+        step = serving.reserve_pages(t, dev(lens, torch.int32), dev(new, torch.int32), ring_d, dev(free, torch.int64),
+                                     page_size=page, max_tokens=total)
+        got = (step.slots, step.positions, step.q_start, step.kv_len, step.free_state, step.granted, t, ring_d)
+        for g, w in zip(got, want):
+            np.testing.assert_array_equal(g.cpu().numpy(), np.asarray(w).astype(g.cpu().numpy().dtype))
+
+
+def test_reserve_of_many_requests_from_several_threads():
+    from concurrent.futures import ThreadPoolExecutor
+
+    def work(requests):
+        zeros, ones = (torch.full((requests,), x, dtype=torch.int32, device="cuda") for x in (0, 1))
+        ring, free = torch.arange(requests, dtype=torch.int32, device="cuda"), dev([0, requests], torch.int64)
+        table = torch.zeros(requests, 1, dtype=torch.int32, device="cuda")
+        for _ in range(200):
+            step = serving.reserve_pages(table, zeros, ones, ring, free, page_size=16, max_tokens=requests)
+        return bool((step.slots == 16 * torch.arange(requests, device="cuda")).all())
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, (6145, 16384, 9000, 16384)))
+
+
 def test_reserve_reports_a_broken_ring_and_bad_lengths():
     def run(lens, new, state, cap=4):
         status = torch.zeros(1, dtype=torch.int32, device="cuda")
