@@ -660,10 +660,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NB)) attend_kernel(const
             kslot = next;
         }
 
-        if (dead) {  // leave the copies still under way the time to land before their places are used again
+        // One warp gave up: the CTA leaves, so that no further wait of its share can run out as well.  The copies that this
+        // warp asked for get the time to land first, and the join finds no task written down.
+        if (dead) {
             const uint64_t start = tc::globaltimer();
             while (tc::globaltimer() - start < tc::kTimeoutNs) {
             }
+        }
+        if (__syncthreads_or(dead)) {
+            if (threadIdx.x == 0) cut->pieces = 0;
+            return;
         }
 
         // -- join the warps: M and l first, then O through the ring, which every warp is done with --
@@ -688,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NB)) attend_kernel(const
         constexpr int V = DP / 32;           // per lane
 #pragma unroll
         for (int h = 0; h < L::kParts; ++h) {
-            __syncthreads();
+            if (h > 0) __syncthreads();
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
