@@ -112,7 +112,8 @@ int attend_of(const ptowsp_kv8_cache* cache, const ptowsp_kv8_attention_args* g,
     a->heads = g->num_heads;
     a->group = g->num_heads / a->cache.kv_heads;
     a->max_q = g->max_q;
-    a->window = g->window;
+    // a window as long as the table hides nothing
+    a->window = g->window < static_cast<int64_t>(g->max_pages) * a->cache.page_size ? g->window : 0;
     a->tokens = g->tokens;
     a->scale = g->scale;
     a->workspace = static_cast<char*>(g->workspace);

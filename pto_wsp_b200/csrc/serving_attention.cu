@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NB)) attend_kernel(const
             const int high = p.q.len - p.q.nq + (row_base + rows - 1) / a.group;  // the last row's
             const int end = min(tok1, low + 1);
             plains = end - kTile >= first ? (end - kTile - first) / kUnit + 1 : 0;
-            if (a.window > 0 && high - a.window >= first) {
+            if (a.window > 0 && high >= a.window && high - a.window >= first) {
                 plain0 = (high - a.window - first) / kUnit + 1;
                 plains = max(plains - plain0, 0);
             }

@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kListThreads) list_kernel(const __grid_constan
             t.base = q.len - q.nq;
             const int first = t.base + t.row0 / a.group, last = t.base + (t.row0 + t.rows - 1) / a.group;
             t.hi = max(0, min(q.len, last + 1));
-            if (a.window > 0 && first - a.window + 1 > 0) t.seen = first - a.window + 1;
+            if (a.window > 0 && first >= a.window) t.seen = first - a.window + 1;  // first may be far below zero
             t.lo = t.seen & ~15;
             t.units = t.hi > t.lo ? (t.hi - t.lo + kKeys - 1) / kKeys : 1;  // a task without keys writes its zeros
             mine = static_cast<int64_t>(t.units) * a.cache.kv_heads;
@@ -545,10 +545,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             const int tile_rows = min(128, w.p.rows - x * 128);
             const int low = w.p.base + (w.p.row0 + x * 128) / a.group;
             const int high = w.p.base + (w.p.row0 + x * 128 + tile_rows - 1) / a.group;
+            const int plain0 = a.window > 0 && high >= a.window ? high - a.window + 1 : 0;
             float M = kNone, l = 0.f;  // l: of this thread's keys
             int key0 = w.p.lo + w.unit0 * kKeys;
             for (int j = 0; j < w.n; ++j, key0 += kKeys) {
-                const bool plain = key0 + kKeys <= min(low + 1, w.p.hi) && (a.window == 0 || key0 > high - a.window);
+                const bool plain = key0 + kKeys <= min(low + 1, w.p.hi) && key0 >= plain0;
                 const float* sc = scales + (steps & 3) * 24 + half * 4;
                 // The scores being there, the step's scales are.  The TMEM loads are the whole warp's.
                 ok = __all_sync(~0u, wait_for(s_full + 8 * x, tiles & 1, abort_flag, a.status));
@@ -557,8 +558,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 ++steps;
                 ++tiles;
                 if (!plain) {  // -inf over what the row does not see
-                    const int c1 = min(pos, w.p.hi - 1) - key0 - half * 64;
-                    const int c0 = a.window > 0 ? pos - a.window + 1 - key0 - half * 64 : -64;
+                    const int k0 = key0 + half * 64, c1 = min(pos, w.p.hi - 1) - k0;
+                    const int c0 = a.window > 0 ? max(pos - k0, 0) - a.window + 1 : -64;  // c1 < 0 hides all of it anyway
 #pragma unroll 1
                     for (int h = 0; h < 4; ++h) {
                         uint32_t r[16];

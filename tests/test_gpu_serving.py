@@ -641,6 +641,15 @@ def test_attend_rows_without_any_request():
             serving.attend_kv8(q, k, v, ks, vs, made[1][:0], none)
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 5, 2 ** 30, 600])
+@pytest.mark.parametrize("lens,qs", [([300, 20, 130, 1], [40, 37, 138, 5]), ([5, 60, 2], [8, 3, 5])])
+def test_attend_windows_longer_than_the_history(window, lens, qs):
+    # with requests of more rows than tokens, whose first rows see nothing
+    out, lse = attend_case("e4m3", torch.float16, 1, 2, 128, 16, lens, qs, window)
+    plain, plain_lse = attend_case("e4m3", torch.float16, 1, 2, 128, 16, lens, qs)
+    assert torch.equal(out, plain) and torch.equal(lse, plain_lse)
+
+
 def test_attend_offsets_beyond_32_bits():
     pages, page, heads, dim = 140_000, 16, 8, 128  # 2.3e9 codes
     gen = torch.Generator(device="cuda").manual_seed(6)
