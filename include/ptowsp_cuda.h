@@ -295,8 +295,8 @@ typedef struct ptowsp_reserve_args {
 PTOWSP_API int ptowsp_cuda_reserve_pages(const ptowsp_reserve_args* args, void* stream);
 
 /* A paged KV cache in 8 bits: codes [num_pages][page_size][num_kv_heads][head_dim] of K and of V with any page, token
- * and head strides (in elements; multiples of 16, codes 16-byte aligned, head_dim contiguous), and one f32 scale per
- * page and head, [num_pages][num_kv_heads]: value = code * scale.  Scales are within 2^-60 .. 2^60.
+ * and head strides (in elements; multiples of 16, codes 16-byte aligned, head_dim contiguous; here and below the stride
+ * of a dimension of one element may be anything), and one f32 scale per page and head, [num_pages][num_kv_heads]: value = code * scale.  Scales are within 2^-60 .. 2^60.
  * page_size: 16, 32, 64 or 128; head_dim: 64 or 128. */
 typedef struct ptowsp_kv8_cache {
     void* k;

@@ -35,6 +35,9 @@ int launched(cudaError_t e, const char* what) noexcept {
 
 bool aligned(const void* p, uintptr_t n) noexcept { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+// Whether a dimension of `n` elements may have this stride: a multiple of `unit`, or any where no second element is.
+bool steps_by(int64_t n, int64_t stride, int64_t unit) noexcept { return n <= 1 || stride % unit == 0; }
+
 bool power_of_two(int64_t v) noexcept { return v > 0 && (v & (v - 1)) == 0; }
 
 // SMs of the current device, asked once per device.
@@ -65,10 +68,13 @@ int kv8_of(const ptowsp_kv8_cache* c, Kv8* out, const char* what) noexcept {
         return fail(PTOWSP_ERR_ARG, "%s: num_kv_heads must be 1 .. 65535 and num_pages 1 .. 2^31 - 1", what);
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
         return fail(PTOWSP_ERR_ARG, "%s: cache codes must be 16-byte aligned, scales 4-byte", what);
-    const int64_t strides[] = {c->k_page_stride, c->k_token_stride, c->k_head_stride,
-                               c->v_page_stride, c->v_token_stride, c->v_head_stride};
-    for (int64_t s : strides)
-        if (s < 0 || (s & 15)) return fail(PTOWSP_ERR_ARG, "%s: cache strides must be multiples of 16, not negative", what);
+    const struct {
+        int64_t n, stride;
+    } dims[] = {{c->num_pages, c->k_page_stride}, {c->page_size, c->k_token_stride}, {c->num_kv_heads, c->k_head_stride},
+                {c->num_pages, c->v_page_stride}, {c->page_size, c->v_token_stride}, {c->num_kv_heads, c->v_head_stride}};
+    for (const auto& d : dims)
+        if (!steps_by(d.n, d.stride, 16) || (d.n > 1 && d.stride < 0))
+            return fail(PTOWSP_ERR_ARG, "%s: cache strides must be multiples of 16, not negative", what);
     int shift = 4;
     while ((1 << shift) < c->page_size) ++shift;
     *out = Kv8{{static_cast<uint8_t*>(c->k), c->k_scale, c->k_page_stride, c->k_token_stride, c->k_head_stride},
@@ -163,8 +169,10 @@ int ptowsp_cuda_kv8_append(const ptowsp_kv8_cache* cache, const ptowsp_kv8_appen
     if (g->tokens == 0) return PTOWSP_OK;
     if (!g->k || !g->v || !g->slots) return fail(PTOWSP_ERR_ARG, "%s: null pointer", what);
     const int64_t unit = g->dtype == PTOWSP_F32 ? 4 : 8;  // elements in 16 bytes
-    if (!aligned(g->k, 16) || !aligned(g->v, 16) || g->k_token_stride % unit || g->k_head_stride % unit ||
-        g->v_token_stride % unit || g->v_head_stride % unit)
+    const int64_t heads = a.cache.kv_heads;
+    if (!aligned(g->k, 16) || !aligned(g->v, 16) || !steps_by(g->tokens, g->k_token_stride, unit) ||
+        !steps_by(heads, g->k_head_stride, unit) || !steps_by(g->tokens, g->v_token_stride, unit) ||
+        !steps_by(heads, g->v_head_stride, unit))
         return fail(PTOWSP_ERR_ARG, "%s: rows of k and v must be 16-byte aligned", what);
     a.k = g->k;
     a.v = g->v;
@@ -196,8 +204,9 @@ int ptowsp_cuda_kv8_attention(const ptowsp_kv8_cache* cache, const ptowsp_kv8_at
         return fail(PTOWSP_ERR_ARG, "%s: null pointer", what);
     if (!a.q_start && (a.tokens != a.requests || a.max_q != 1))
         return fail(PTOWSP_ERR_ARG, "%s: without q_start every request has one token (max_q 1)", what);
-    if (!aligned(a.q, 16) || !aligned(a.out, 16) || a.q_token_stride % 8 || a.q_head_stride % 8 ||
-        a.out_token_stride % 8 || a.out_head_stride % 8)
+    if (!aligned(a.q, 16) || !aligned(a.out, 16) || !steps_by(a.tokens, a.q_token_stride, 8) ||
+        !steps_by(a.heads, a.q_head_stride, 8) || !steps_by(a.tokens, a.out_token_stride, 8) ||
+        !steps_by(a.heads, a.out_head_stride, 8))
         return fail(PTOWSP_ERR_ARG, "%s: rows of q and out must be 16-byte aligned", what);
     int sms = 0;
     rc = sm_count(&sms);

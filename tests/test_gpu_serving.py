@@ -650,6 +650,28 @@ def test_attend_windows_longer_than_the_history(window, lens, qs):
     assert torch.equal(out, plain) and torch.equal(lse, plain_lse)
 
 
+def test_strides_of_dimensions_of_one_element():
+    # one page, one head, one token: nothing steps by their strides, whatever they are
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    fill = lambda *size: torch.randn(size, generator=gen, device="cuda")  # noqa: E731
+    odd = lambda t: torch.as_strided(t, (1, *t.shape), (1027, *t.stride()))  # noqa: E731
+    for dtype in (torch.float16, torch.float32):
+        kc, vc = (torch.zeros(16, 128, dtype=torch.int8, device="cuda") for _ in range(2))
+        kc, vc = (torch.as_strided(c, (1, 16, 1, 128), (5, 128, 3, 1)) for c in (kc, vc))
+        ks, vs = (torch.ones(1, 1, device="cuda") for _ in range(2))
+        k, v = fill(2, 1, 1, 128).to(dtype)
+        k, v = (torch.as_strided(x, (1, 1, 128), (7, 5, 1)) for x in (k, v))
+        serving.append_kv8(k, v, dev([0], torch.int64), kc, vc, ks, vs)
+        assert torch.allclose(kc[0, 0].float() * ks, k[0].float(), atol=0.02)
+        assert torch.allclose(vc[0, 0].float() * vs, v[0].float(), atol=0.02)
+        for group in (1, 4):
+            q, out = (odd(fill(group, 128).half()) for _ in range(2))
+            if group == 1:
+                q, out = (torch.as_strided(x, (1, 1, 128), (3, 5, 1)) for x in (q, out))
+            got = serving.attend_kv8(q, kc, vc, ks, vs, dev([[0]], torch.int32), dev([1], torch.int32), out=out)
+            assert torch.allclose(got.float(), (vc[0, 0].float() * vs).expand(1, group, 128), atol=1e-2)
+
+
 def test_attend_offsets_beyond_32_bits():
     pages, page, heads, dim = 140_000, 16, 8, 128  # 2.3e9 codes
     gen = torch.Generator(device="cuda").manual_seed(6)
