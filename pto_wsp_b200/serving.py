@@ -12,7 +12,8 @@ They call the C entry points ``ptowsp_cuda_reserve_pages``, ``_kv8_append``, ``_
 ``ValueError`` here, or :class:`~pto_wsp_b200.runtime.PtoWspCudaError` with the library's status.  What only the device
 sees (a page id outside the cache, a request without room) is or'ed into the ``status`` tensor, an int32 that the caller
 zeroes; :func:`check_status` reads it and raises.  The calls allocate their results (and the attention its workspace)
-with torch's allocator on the current stream, and keep nothing.
+with torch's allocator on the current stream, and keep nothing.  They have no gradient: inputs that require one are
+refused (``ValueError``) unless gradients are off, as under ``torch.no_grad()``.
 """
 
 from __future__ import annotations
@@ -109,6 +110,11 @@ def _call(fn, index, *structs):
 def _need(cond, text):
     if not cond:
         raise ValueError(text)
+
+
+def _no_gradient():
+    if torch.is_grad_enabled():
+        raise ValueError("the serving operators have no gradient: call them under torch.no_grad(), or detach the inputs")
 
 
 def _cuda_index(t, name):
@@ -209,6 +215,8 @@ def append_kv8(k, v, slots, k_cache, v_cache, k_scale, v_scale, *, status=None) 
     has one float32 scale per page and head.  A page's scale grows with its tokens, and its earlier codes are then
     rounded again; writing a page's first token begins its scale anew."""
     index, cache, heads, dim = _cache(k_cache, v_cache, k_scale, v_scale)
+    if k.requires_grad or v.requires_grad:
+        _no_gradient()
     tokens = k.shape[0]
     dtype = _DTYPES.get(k.dtype)
     if dtype is None or v.dtype is not k.dtype:
@@ -234,6 +242,8 @@ def attend_kv8(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_len, *, q_s
     window - 1 before it.  Returns out like q, and with ``return_lse`` also float32 [tokens, heads].  Rows that see no
     key, that no request has, or whose request has more than ``max_q`` (also reported) are zeros with an lse of -inf."""
     index, cache, _, dim = _cache(k_cache, v_cache, k_scale, v_scale)
+    if q.requires_grad:
+        _no_gradient()
     dtype = _DTYPES.get(q.dtype)
     if not dtype:
         raise TypeError(f"q must be float16 or bfloat16 (got {q.dtype})")
@@ -279,6 +289,8 @@ def sample_tokens(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=
     Returns the tokens, int32 [rows] (-1 where every logit is -inf or NaN), and the logarithm of each one's
     probability among what the settings left, float32 [rows]."""
     index = _cuda_index(logits, "logits")
+    if logits.requires_grad:
+        _no_gradient()
     dtype = _DTYPES.get(logits.dtype)
     if dtype is None:
         raise TypeError(f"logits must be float32, float16 or bfloat16 (got {logits.dtype})")

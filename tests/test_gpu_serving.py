@@ -711,6 +711,23 @@ def test_attend_refusals():
         serving.attend_kv8(q, k, v, ks, vs, table, n, out=torch.empty(2, 4, 64, device="cuda").half())
 
 
+def test_inputs_that_require_a_gradient():
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    (k, ks), (v, vs) = (made := paged("int8", [20], 16, 2, 64, "nhd", gen))[0]
+    q, x, n, u = torch.randn(1, 4, 64).half(), torch.randn(1, 2, 64), dev([20], torch.int32), torch.rand(1, device="cuda")
+    q, x, logits = (t.cuda().requires_grad_() for t in (q, x, torch.randn(1, 50)))
+    calls = (lambda: serving.attend_kv8(q, k, v, ks, vs, made[1], n), lambda: serving.sample_tokens(logits, u),
+             lambda: serving.append_kv8(x, x.detach(), dev([0], torch.int64), k, v, ks, vs),
+             lambda: serving.append_kv8(x.detach(), x, dev([0], torch.int64), k, v, ks, vs))
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+        with torch.inference_mode():
+            call()
+
+
 # ---------------------------------------------------------------------------
 # sample_tokens
 # ---------------------------------------------------------------------------
