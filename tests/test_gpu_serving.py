@@ -871,3 +871,77 @@ def test_sample_shares_follow_the_distribution():
     token, _ = serving.sample_tokens(x, u)
     share = torch.bincount(token.long(), minlength=vocab).double()
     assert float((share - torch.softmax(x[0].double(), 0) * rows).abs().max()) <= 1.001
+
+
+def test_a_whole_step_in_a_graph():
+    # reserve, append, attend and sample captured once and replayed, the state in place, against the same calls one by one
+    requests, heads, group, dim, vocab, page, steps = 5, 2, 4, 64, 700, 16, 40
+    gen = torch.Generator(device="cuda").manual_seed(14)
+    most = 12  # rows of a step: fewer are used, the rest is padding
+    x = torch.randn(steps, 3, most, heads * group, dim, generator=gen, device="cuda").half()
+    u = torch.rand(steps, requests, generator=gen, device="cuda")
+    new = torch.randint(0, 3, (steps, requests), generator=gen, device="cuda", dtype=torch.int32)
+    new[17, 2] = new[23, 0] = -1
+    weight = torch.randn(heads * group * dim, vocab, generator=gen, device="cuda").half()
+    top_p = torch.full((requests,), 0.9, device="cuda")
+
+    def state():
+        cache = [torch.zeros(60, heads, page, dim, dtype=torch.int8, device="cuda").transpose(1, 2) for _ in range(2)]
+        return cache + [torch.ones(60, heads, device="cuda") for _ in range(2)], {
+            "table": torch.zeros(requests, 8, dtype=torch.int32, device="cuda"), "ring": torch.arange(60, device="cuda").int(),
+            "len": torch.zeros(requests, dtype=torch.int32, device="cuda"), "free": dev([0, 60], torch.int64),
+            "status": torch.zeros(1, dtype=torch.int32, device="cuda")}
+
+    def step(cache, s, x, new, u):
+        plan = serving.reserve_pages(s["table"], s["len"], new, s["ring"], s["free"], page_size=page, max_tokens=most,
+                                     status=s["status"])
+        serving.append_kv8(x[1][:, :heads], x[2][:, :heads], plan.slots, *cache, status=s["status"])
+        a, lse = serving.attend_kv8(x[0], *cache, s["table"], plan.kv_len, q_start=plan.q_start, max_q=2, return_lse=True,
+                                    status=s["status"])
+        rows = (plan.q_start[1:] - 1).clamp(min=0).long()
+        token, logprob = serving.sample_tokens(a.reshape(most, -1)[rows] @ weight, u, top_p=top_p)
+        s["len"].copy_(plan.kv_len)
+        s["free"].copy_(plan.free_state)
+        return a, lse, token, logprob
+
+    one, other = state(), state()
+    want = [[t.clone() for t in step(*one, x[i], new[i], u[i])] for i in range(steps)]
+    ins = [x[0].clone(), torch.zeros_like(new[0]), u[0].clone()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):  # the calls before have loaded the code
+        got = step(*other, *ins)
+    for i in range(steps):
+        for to, t in zip(ins, (x, new, u)):
+            to.copy_(t[i])
+        graph.replay()
+        for name, w, g in zip(("out", "lse", "token", "logprob"), want[i], got):
+            assert torch.equal(w, g), (i, name)
+        pad = int(new[i].clamp(min=0).sum())
+        assert not got[0][pad:].any()
+    for a, b in zip([*one[0], *one[1].values()], [*other[0], *other[1].values()]):
+        assert torch.equal(a, b)
+    serving.check_status(other[1]["status"])
+
+
+def test_attend_from_several_threads():
+    from concurrent.futures import ThreadPoolExecutor
+
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    cases = []
+    for lens, qs in (([700, 20], [1, 1]), ([500, 300], [70, 1]), ([90, 4000], [3, 5]), ([260, 300], [200, 256])):
+        (k, ks), (v, vs) = (made := paged("e4m3", lens, 16, 2, 128, "hnd", gen))[0]
+        q = torch.randn(sum(qs), 8, 128, generator=gen, device="cuda").half()
+        more = {"q_start": dev(np.cumsum([0] + qs), torch.int32), "max_q": max(qs)}
+        args = (q, k, v, ks, vs, made[1], dev(lens, torch.int32))
+        cases.append((args, more, serving.attend_kv8(*args, **more)))
+    torch.cuda.synchronize()
+
+    def work(case):
+        args, more, want = case
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [serving.attend_kv8(*args, **more) for _ in range(50)]
+            torch.cuda.current_stream().synchronize()
+            return all(torch.equal(g, want) for g in got)
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, cases))

@@ -74,3 +74,42 @@ def test_serving_loop(cache, require_cuda):
     assert tail - head == pages  # every page came back
     at = torch.arange(head, tail) % pages
     assert sorted(server.ring.cpu()[at].tolist()) == list(range(pages))
+
+
+def dequantised_logits(ex, model, server, slot, text):
+    """The model over a whole text in f64, each layer's attention over the K and V that the server's cache holds for it."""
+    pages = server.table[slot, :-(-len(text) // model.page_size)].long()
+    x = (model.embedding[torch.tensor(text, device="cuda")] + model.position[:len(text)]).double()
+    for i, (qkv, out) in enumerate(zip(model.qkv, model.out)):
+        y = (torch.nn.functional.layer_norm(x, x.shape[-1:]) @ qkv.double()).view(len(text), -1, model.dim)
+        k, v = ((c[i][pages].double() * s[i][pages].double()[:, None, :, None]).reshape(-1, model.kv_heads, model.dim)
+                [:len(text)].repeat_interleave(model.heads // model.kv_heads, 1)
+                for c, s in ((model.k, model.k_scale), (model.v, model.v_scale)))
+        s = torch.einsum("qhd,khd->hqk", y[:, :model.heads], k) * model.dim ** -0.5
+        s = s.masked_fill(torch.ones_like(s[0]).triu(1).bool(), float("-inf"))
+        x = x + torch.einsum("hqk,khd->qhd", torch.softmax(s, -1), v).reshape(len(text), -1) @ out.double()
+    return torch.nn.functional.layer_norm(x[-1], x.shape[-1:]) @ model.head.double()
+
+
+@pytest.mark.parametrize("cache", ["e4m3", "int8"])
+def test_serving_loop_logits_follow_from_the_cache(cache, require_cuda):
+    # One token per step into short texts, so that every page's scale counts.  What is left between the two is rounding to
+    # f16 (2^-11) in some six places per layer, none of which a layer norm enlarges: 2^-7 of the logits' norm.  A layer's own
+    # row is written from f16 activations, which the recompute has in f64; that is among the six.
+    ex = example()
+    model = ex.Decoder(12, heads=8, kv_heads=2, dim=64, vocab=512, cache=cache)
+    server = ex.Server(model, 3, 12, 4, chunk=1)
+    prompts = [[5, 9, 300], [17], [400, 2, 2, 511, 30]]
+    for slot, prompt in enumerate(prompts):
+        server.admit(slot, prompt, 30)
+    texts = [[] for _ in prompts]
+    for _ in range(30):
+        fed = [list(w[:1]) for w in server.waiting]
+        logits = server.step(torch.zeros(3, device="cuda"), torch.ones(3, device="cuda"))
+        for slot, new in enumerate(fed):
+            texts[slot] += new
+            if not new:
+                continue
+            want = dequantised_logits(ex, model, server, slot, texts[slot])
+            assert float((logits[slot].double() - want).norm() / want.norm()) < 2.0 ** -7, (slot, len(texts[slot]))
+    serving.check_status(server.status)
