@@ -312,7 +312,8 @@ typedef struct ptowsp_kv8_cache {
 
 /* Writes new K and V rows into the cache.  k, v: [tokens][num_kv_heads][head_dim] of `dtype`, strides in elements,
  * rows 16-byte aligned.  slots: i64 [tokens], page * page_size + offset, -1: skip; the slots of one page stand next to
- * each other in ascending order (as ptowsp_cuda_reserve_pages makes them), and no page belongs to two requests.
+ * each other in ascending order, each once and with no -1 between them (as ptowsp_cuda_reserve_pages makes them), and
+ * no page belongs to two requests: two separate runs of one page would settle its scale side by side, unordered.
  * For each touched page and head, from the largest finite |x| of its new tokens:
  *   need  = the smallest power of two s with max <= 448 s (e4m3), or max * (1 / 127) in f32 (int8), within 2^-60 .. 2^60
  *   scale = max(need, old), or need alone if the page's token 0 is among the new ones (the page is new)

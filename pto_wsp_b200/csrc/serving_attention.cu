@@ -13,7 +13,7 @@
 //
 // Bound by HBM: every code is read once.  64 requests of one token over 512-8192 keys (8 KV heads of 128, groups of four:
 // 582 MB) take 108 us as a whole call, 5.4 TB/s; the copy rate would take 89.  Three requests over 100,000-200,000 keys:
-// 114 us for 599 MB.  What is left is the second launch and the CTAs' ends, some 8 us, and the warps' waits for boxes of
+// 115 us for 599 MB.  What is left is the second launch and the CTAs' ends, some 8 us, and the warps' waits for boxes of
 // 2 to 4 KB, which 16 bytes per thread by cp.async (118 us) and plain loads (128) served worse.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -839,7 +839,11 @@ cudaError_t launch_rows(const AttendArgs& a, int sms, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, join_kernel<D, NB>, a);
 }
 
-// Fragments of 8 q rows per tile.  With requests left to the other kernel most of the rest have one token.
+// Fragments of 8 q rows per tile: as many as the largest request needs, but where the large ones are left to the other
+// kernel, as many as one token does.  That is right where the rest have one token, and wrong where they have several, whose
+// cache is then read once per tile; the lengths are on the device, so the rule cannot tell.  Whole calls with tiles of
+// one token / of up to 32 rows, 4096 keys, D = 128: two chunks and 30 single tokens, groups of four, 245 / 259 us; one of 10
+// tokens and 63 single ones 161 / 200; a chunk and 31 of 2-8 tokens 228 / 218; up to 9 tokens each 181 / 159.
 int fragments(const AttendArgs& a) {
     const int64_t rows = a.few ? a.group : static_cast<int64_t>(a.max_q) * a.group;
     return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
@@ -855,8 +859,10 @@ cudaError_t launch_d(const AttendArgs& a, int sms, cudaStream_t s) {
 }
 
 // Above so many q rows of a request and KV head the tcgen05 kernel is faster although it pads them to 128: the warp MMAs
-// read the codes once per 32 rows.  32 requests of 8 KV heads over 4096 keys each: 32 rows take 122 us here and 173
-// there, 40 rows 208 here and 175 there.
+// read the codes once per 32 rows.  Here / there in us, 4096 keys each: 32 requests of 8 KV heads, D = 128, int8 or e4m3: 32
+// rows 114-122 / 169-171, 40 rows 193-208 / 169-173; 8 requests of 2 heads: 46 / 52, then 52 / 52 up to 64 rows; four of 8
+// heads over 32768 keys: 116 / 161, then 181 / 159.  With D = 64 the rows between 33 and 64 would still be faster
+// here (32 requests of 4 heads: 32 rows 63 / 91, 40 rows 81 / 91, 64 rows 85 / 93), which the rule gives away.
 constexpr int kFew = 32;
 
 size_t few_bytes(const AttendArgs& a, int sms) {

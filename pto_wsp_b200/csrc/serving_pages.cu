@@ -13,12 +13,13 @@ namespace {
 // ---------------------------------------------------------------------------
 // Reservation.  Per request r: have = ceil(len / page), need = ceil((len + new) / page) - have; the new pages are the
 // ring entries head + (sum of need before r) + j, the new tokens the list entries q_start[r] + j.  Everything follows
-// from three prefix sums over the requests (tokens, needed pages, returned pages).  Every CTA runs the sums for
-// itself -- a thousand requests are one round of a block scan, cheaper than a second launch -- keeps the two that the
-// token list needs in shared memory and then fills its share of the outputs; CTA 0 writes the per-request ones.
+// from prefix sums over the requests: tokens, needed pages, returned pages, and the pages in fact given, four block scans
+// of three barriers each per 1024 requests.  Every CTA runs the sums for itself -- a thousand requests are one round of
+// the scans, cheaper than a second launch -- keeps the two that the token list needs in shared memory and then fills its
+// share of the outputs; CTA 0 writes the per-request ones.
 //
-// Bound by latency: 6 us on the device for 64 requests of one token, 12 for 1001 requests with 0-511 each, of a whole call
-// of 18 us in which the host allocates six results.
+// Bound by latency: 5.5 us on the device for 64 requests of one token, 12 for 1001 requests with 0-511 each, of a whole
+// call of 18 us in which the host allocates six results.
 // ---------------------------------------------------------------------------
 
 constexpr int kRsvThreads = 1024;
@@ -32,7 +33,7 @@ __device__ __forceinline__ int64_t warp_inclusive(int64_t v, int lane) {
     return v;
 }
 
-// Inclusive scan over the block; *total: the block's sum.  `part`: 33 words that nothing else uses.
+// Inclusive scan over the block; *total: the block's sum.  `part`: 32 words that nothing else uses.
 __device__ __forceinline__ int64_t block_inclusive(int64_t v, int64_t* part, int64_t* total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     v = warp_inclusive(v, lane);
@@ -172,8 +173,9 @@ __global__ void __launch_bounds__(kRsvThreads) reserve_kernel(ReserveArgs a) {
 // each; few long ones (prefill): the warps share each, so that its rows are all under way at once and are read once.
 //
 // Bound by HBM in principle, 2 or 4 bytes in and 1 out per element; in fact by instructions and the runs' fixed parts:
-// 16,001 tokens of 8 heads of 128 in f16 to int8 (98 MB) take 46 us, 2.1 TB/s, of which rounding is a sixth.  One warp
-// per run took 128 us there.  64 single tokens take 8.5 us, 4.4 of them on the device.
+// 16,001 tokens of 8 heads of 128 in f16 to int8 (98 MB) take 45 us, 2.2 TB/s, and 31 million warp instructions.  Without
+// the encoding it would be 23 million and a sixth less time: the rest is addresses, slots, bookkeeping, and warps that wait at
+// the barrier while the first one looks for runs.  One warp per run took 128 us there.  64 single tokens take 8.5 us, 4.4 of them on the device.
 // ---------------------------------------------------------------------------
 
 constexpr int kAppWarps = 8;

@@ -20,10 +20,11 @@
 // TMEM: S_A, S_B (128 columns each; P over the first 32 of either half), O_A, O_B.  The tensor pipe runs one thread's MMAs
 // in order, so S' may follow PV into the columns that P is read from, and S' being done means that PV is.
 //
-// Bound by the tensor pipe's feed and by the chain score - softmax - product of a tile.  Chunks of 1142-1516 rows over
-// 2791-6204 keys (8 KV heads, groups of four, D = 128: 355 GFLOP) take 553 us, 643 TFLOP/s; both products of a step take
-// 2048 cycles at the full rate and some 3000 here, seen from the issuing thread: Q and K tiles, the conversion and the
-// copies share shared memory's 128 bytes a cycle.  The rest is the chain's, and a CTA's way from one task to the next.
+// Bound by the chain score - softmax - product of a tile, beside which the tensor pipe stands idle for two thirds of the
+// time.  Chunks of 1142-1516 rows over 2791-6204 keys (8 KV heads, groups of four, D = 128: 355 GFLOP) take 541 us, 656
+// TFLOP/s, as a whole call.  Of the main kernel's 906 thousand cycles (148 steps a CTA, 6100 a step) the tensor pipe works
+// 34 %, the 2048 that both products of a step take at the full rate; instructions issue in 56 % of the cycles.  The
+// list takes 7 us, the join 25 and the few-rows kernel and its join 23, one after the other and cold.
 //
 // Work is dealt out as for few rows: the steps of all (tile pair, head) tasks stand in one line, every CTA takes an equal
 // part, and tasks that this cuts are joined by a second launch.  A first launch lists the tile pairs.
@@ -451,8 +452,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         // Rows of q and of the output go between memory and this tile's place in shared memory with kRowLanes lanes side by
         // side in a row; two warps share 32 rows, 16 each.  These loops and the converters' are rolled up on purpose: the
         // roles' code has to stay in the instruction cache together.  For chunks of 1100-1500 rows over 2800-6200 keys
-        // (21864 steps) both rolled take 553 us; the converters unrolled over K and V 610, these loops unrolled as well 700.
-        // The softmax's inner loops lose when rolled up (568), and so does the MMA thread's over the two tiles (590).
+        // (21864 steps) both rolled take 543 us; the converters unrolled over K and V 596, these loops unrolled as well 616.
+        // The softmax's inner loops lose when rolled up (558), and so does the MMA thread's over the two tiles (569).
         constexpr int kRowLanes = D / 8, kRowsRead = 32 / kRowLanes;
         const auto io_lane = []() {  // read anew at either use: what follows from it would hold registers across the steps
             int i;

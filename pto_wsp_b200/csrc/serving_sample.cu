@@ -13,9 +13,11 @@
 // over its range of composites.
 //
 // Bound by a row's chain of barriers: a pass over a slice in shared memory takes about a microsecond, and each pass waits
-// for the one before.  One row of 50,021 (top-p) takes 26 us, 64 rows of 131,072 with all filters 29 us (17 MB, 0.6
-// TB/s), 509 rows of 32,000 without filters 37.6 us (65 MB, 1.7 TB/s).  Two rows in flight per cluster took 60 for the
-// last, slices read from L1 and L2 instead of shared memory 37-52.
+// for the one before.  One row of 50,021 (top-p) takes 15 to 43 us on the device: 15 to 22 where the counts leave no
+// more candidates than can be ranked at once, 32 to 43 where the window has to be summed by mass, as in 14 of 24 drawn
+// rows.  64 rows of 131,072 with all filters take 29 us as a whole call (17 MB, 0.6 TB/s), 509 rows of 32,000 without filters 37.6 (65 MB,
+// 1.7 TB/s).  Two rows in flight per cluster took 60 for the last, slices read from L1 and L2 instead of shared memory
+// 37-52.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -768,9 +770,11 @@ cudaError_t launch_cluster(const SampleArgs& a, int sms, cudaStream_t s) {
     const auto slice_of = [&](int cl) { return ((a.vocab + cl - 1) / cl + 7) & ~7; };
     const auto bytes_of = [&](int cl) { return slice_of(cl) * static_cast<int64_t>(sizeof(T)) + 16 + extra; };
     const auto per_sm = [&](int cl) { return std::min<int64_t>(CUTS ? 2 : 3, (227 << 10) / (bytes_of(cl) + 2048)); };
-    // Slices of 8000 elements or more: below that the cluster's barriers and remote reads cost more than the passes save
-    // (one row of 8000 with top-p: 7.5 us in one CTA, 10.9 in four, 16.9 in eight; of 50000: 112, 44, 47).  Few rows are
-    // spread over the SMs, one CTA each; many rows share them, so that one is read while another is worked on.
+    // Slices of 8000 elements or more: below that the cluster's barriers and remote reads cost what the passes save, or more.
+    // One row with top-p in 1, 2, 4 and 8 CTAs, device us: of 8000 10.5, 10.8, 10.8, 12.8; of 16000 13.4, 12.3, 11.4, 13.3
+    // (taken: two); of 32000 20.4, 16.4, 13.7, 14.8; of 50000 28.4, 21.3, 16.6, 16.9, and 70, 46, 32, 30 where its window has
+    // to be summed; of 131072 24.8 in four and 21.4 in eight, 81 and 55 with the window.  Few rows are spread over the SMs, one CTA
+    // each; many rows share them, so that one is read while another is worked on.
     int cl = 1;
     while (cl < kMaxCluster && (slice_of(cl) > 32768 || bytes_of(cl) > kSampleMaxSmem ||
                                 (static_cast<int64_t>(a.rows) * cl * 2 <= sms && slice_of(cl * 2) >= 8000) ||

@@ -209,7 +209,7 @@ def _cache(k_cache, v_cache, k_scale, v_scale):
 
 def append_kv8(k, v, slots, k_cache, v_cache, k_scale, v_scale, *, status=None) -> None:
     """Write the rows ``k``, ``v`` [tokens, heads, head_dim] (float32, float16 or bfloat16) into the cache at ``slots``
-    (int64 [tokens], -1: skip; those of one page next to each other and ascending).
+    (int64 [tokens], -1: skip; those of one page next to each other and ascending, none twice and no -1 between them).
 
     The cache, codes [pages, page_size, heads, head_dim] in float8_e4m3fn or int8 with any page, token and head order,
     has one float32 scale per page and head.  A page's scale grows with its tokens, and its earlier codes are then
