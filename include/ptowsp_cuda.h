@@ -341,8 +341,9 @@ PTOWSP_API int ptowsp_cuda_kv8_append(const ptowsp_kv8_cache* cache, const ptows
  *   max_q       the most rows that any request has; one with more is left out and reported
  *   window      > 0: a row sees its own token and the window - 1 before it; 0: all before it
  * Row j of nq sees the keys t <= kv_len - nq + j.  A row that sees none gets zeros and lse = -inf, and so does one that
- * no request has or whose request is left out.  A page id outside the cache hides its tokens.  `workspace`: ptowsp_cuda_kv8_attention_workspace bytes, 256-byte aligned,
- * contents irrelevant, used until the call's work on the stream is done. */
+ * no request has or whose request is left out.  A page id outside the cache hides its tokens.
+ * `workspace`: ptowsp_cuda_kv8_attention_workspace bytes, 256-byte aligned, contents irrelevant, used until the call's
+ * work on the stream is done. */
 typedef struct ptowsp_kv8_attention_args {
     const void* q;
     void* out;
@@ -366,8 +367,8 @@ PTOWSP_API int ptowsp_cuda_kv8_attention(const ptowsp_kv8_cache* cache, const pt
 PTOWSP_API size_t ptowsp_cuda_kv8_attention_workspace(const ptowsp_kv8_cache* cache,
                                                       const ptowsp_kv8_attention_args* args);
 
-/* One token per row of logits [rows][vocab] (f32, f16 or bf16; rows `row_stride` elements apart; vocab up to 393216), from one uniform
- * random number u[row] in [0, 1) each.  With the row's largest logit M, w_i = exp((x_i - M) / temperature), taken as a
+/* One token per row of logits [rows][vocab] (f32, f16 or bf16; rows `row_stride` elements apart; vocab up to 393216), from
+ * one uniform random number u[row] in [0, 1) each.  With the row's largest logit M, w_i = exp((x_i - M) / temperature), taken as a
  * whole number of 2^-40 (so its sums do not depend on their order).  Ordered by falling logit, ties by rising index,
  * the candidates are cut to the first top_k, to w_i >= min_p, and then to the shortest prefix that holds top_p of what
  * is left; the token is the first candidate, by index, at which the running sum of w passes u times the sum.
